@@ -100,6 +100,14 @@ def _load():
         'asr_device_bytes': (i64, [vp]),
         'asr_range_retries': (i64, [vp]),
         'asr_crc32c': (C.c_uint32, [vp, i64, C.c_uint32]),
+        # operators on device memory: the argument struct as bytes (asr_amd/ops.py packs it), the stream
+        'asr_ops_last_error': (C.c_char_p, []),
+        'asr_token_logprobs': (i32, [C.c_char_p, vp]),
+        'asr_cross_attention': (i32, [C.c_char_p, vp]),
+        'asr_cross_attention_workspace': (i64, [i32] * 7),
+        'asr_kv8_append': (i32, [C.c_char_p, vp]),
+        'asr_kv8_attention': (i32, [C.c_char_p, vp]),
+        'asr_kv8_attention_workspace': (i64, [i32] * 7),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -12,8 +12,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')
 LIB = os.path.join(CSRC, 'libasr_amd.so')
-SOURCES = ['gemm_f32.hip', 'gemm_split.hip', 'rowops.hip', 'frontend.hip', 'attention.hip', 'engine.hip']
-HEADERS = ['asr_common.h', 'gemm_epilogue.h', os.path.join('..', '..', 'include', 'asr_amd.h')]
+SOURCES = ['gemm_f32.hip', 'gemm_split.hip', 'rowops.hip', 'frontend.hip', 'attention.hip', 'ops_rows.hip', 'ops_attention.hip', 'engine.hip']
+HEADERS = ['asr_common.h', 'gemm_epilogue.h', 'ops_common.h', os.path.join('..', '..', 'include', 'asr_amd.h')]
 # Packed float32 instructions are off: the compiler makes them from ordinary float code, and some of their forms have given wrong
 # results on this hardware.  (The host pass does not know the feature and warns; that is harmless.)
 FLAGS = ['-O3', '-std=c++17', '--offload-arch=gfx950', '-fPIC', '-Wall', '-Wno-unused-function',

@@ -1,0 +1,612 @@
+// Attention operators on device memory: over the states of another sequence, and over the 8-bit K/V cache.  C entry points:
+// include/asr_amd.h.
+//
+// With G = heads / kv_heads, the rows r = i * G + g of one (sequence, K/V head) share its keys and values:
+//     S = c q K^T,   P = e^(S - m),   out = P V / l,   m = running row maximum, l = running row sum of P
+// taken over tiles of keys in one pass (when m grows, what was summed is scaled by e^(m_old - m_new)).  Everything is computed transposed:
+// S^T = K q^T leaves a query row in each lane of 16 (its statistics are then per-lane values and need no exchange but over the four lane
+// groups), and O^T = V^T P^T takes the probabilities straight from the accumulators as its second operand: the order of keys inside a tile is
+// free, so tile row m is given the key that puts eight consecutive keys of one lane group where the next product wants them.
+#include "ops_common.h"
+
+#include <math.h>
+
+namespace {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float NEG_INF = -__builtin_inff();
+
+enum { KV_F32 = ASR_F32, KV_BF16 = ASR_BF16, KV_F16 = ASR_F16, KV_E4M3 = 3 };
+
+struct AttnArgs {
+    const char *q, *k, *v;
+    char* out;
+    const float *k_scale, *v_scale;      // KV_E4M3
+    const int32_t* lens;
+    const uint8_t* pad;
+    float* ws;                           // nsplit > 1: per (split, sequence, K/V head, row): m, l, then O [d]
+    int64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3];        // bytes; of n, t, head
+    int64_t pad_stride, scale_stride;    // scale_stride: floats of one (sequence, head)
+    int n, tq, tk, kv_heads, group, d, causal;
+    int rows, tiles, nsplit;             // rows = tq * group of one (sequence, K/V head); tiles of rows
+    float c;                             // scale * log2(e): powers of two instead of e
+};
+
+__device__ inline uint32_t pack_bf16(float a, float b)
+{
+    bf16x2 r;
+    r[0] = (__bf16)a;
+    r[1] = (__bf16)b;
+    return __builtin_bit_cast(uint32_t, r);
+}
+__device__ inline uint32_t pack_f16(float a, float b)
+{
+    f16x2 r;
+    r[0] = (_Float16)a;
+    r[1] = (_Float16)b;
+    return __builtin_bit_cast(uint32_t, r);
+}
+template <bool F16> __device__ inline uint32_t pack16(float a, float b) { return F16 ? pack_f16(a, b) : pack_bf16(a, b); }
+template <bool F16> __device__ inline f32x2 unpack16(uint32_t u)
+{
+    f32x2 r;
+    if (F16) {
+        const f16x2 h = __builtin_bit_cast(f16x2, u);
+        r[0] = (float)h[0];
+        r[1] = (float)h[1];
+    } else {
+        r[0] = __uint_as_float(u << 16);
+        r[1] = __uint_as_float(u & 0xffff0000u);
+    }
+    return r;
+}
+template <bool F16> __device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c)
+{
+    if (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// two e4m3 codes (the low or the high half of a word) times a power of two: exact in bf16
+template <bool HI> __device__ inline uint32_t codes_bf16(uint32_t w, float scale)
+{
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, HI));
+}
+
+// maximum / sum over the four 16-lane groups of a wave
+__device__ inline float groups_max(float x)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float groups_sum(float x)
+{
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// e^(m_old - m_new) as a power of two of the scaled scores; 0 where nothing was summed yet
+__device__ inline float rescale(float m_old, float m_new) { return m_old == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_old - m_new); }
+
+__device__ inline int keys_of(const AttnArgs& a, int b) { return a.lens ? min(max(a.lens[b], 0), a.tk) : a.tk; }
+
+// ---- few rows: the waves of a workgroup share the keys ------------------------------------------------------------------
+// A workgroup has one tile of 16 NQ rows of one (sequence, K/V head) and one share of its keys; its four waves take 32 keys at a time in turn,
+// straight from memory into registers in the operands' own order (no LDS in the loop), and join their sums in LDS at the end.  K and V are
+// read once by each row tile: bound by those bytes while there are few rows.  QT: type of q and out, KVT: of K and V.
+// Terms: 16-bit K / V are exact factors; q enters as QTERMS 16-bit terms (bf16 codes: f16 = 2, f32 = 3 bf16 terms lose nothing) and
+// P as PTERMS (two: 2^-17 / 2^-22 of it lost, three: nothing), which costs matrix instructions that a loop waiting for memory has to spare.
+template <int QT, int KVT, int DP, int NQ> struct Few {
+    static constexpr bool MATH32 = KVT == KV_F32, F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
+    static constexpr int QTERMS = CODES ? (QT == ASR_F32 ? 3 : QT == ASR_F16 ? 2 : 1) : 1;
+    static constexpr int PTERMS = CODES && QT == ASR_F32 ? 3 : 2;
+    static constexpr int KVB = KVT == KV_F32 ? 4 : CODES ? 1 : 2;         // bytes of a K / V value
+    static constexpr int QB = QT == ASR_F32 ? 4 : 2;
+    static constexpr int KW = DP / 4 * KVB / 4;                             // words of a key row in one lane (a quarter of it)
+    static constexpr int VW = DP / 16 * KVB / 4;                            // words of a value row in one lane (a sixteenth)
+    static constexpr int NO = DP / 16;                                      // 16 x 16 output tiles of one row tile
+};
+
+constexpr int FEW_WAVES = 4;
+
+// the place in a row of value j (0 .. DP/4) of lane group g's quarter of it
+template <int KVT> __device__ constexpr int quarter_at(int g, int j)
+{
+    return KVT == KV_F32 ? 16 * (j >> 2) + 4 * g + (j & 3) : KVT == KV_E4M3 ? 64 * (j >> 4) + 16 * g + (j & 15) : 32 * (j >> 3) + 8 * g + (j & 7);
+}
+
+template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW_WAVES) void attention_few_kernel(AttnArgs a)
+{
+    typedef Few<QT, KVT, DP, NQ> F;
+    constexpr int PITCH = DP + 4;
+    __shared__ float s_m[FEW_WAVES][16 * NQ], s_l[FEW_WAVES][16 * NQ];
+    __shared__ __align__(16) float s_o[FEW_WAVES][16 * NQ][PITCH];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x16 = lane & 15, g = lane >> 4;
+    int64_t id = blockIdx.x;
+    const int bh = (int)(id % ((int64_t)a.n * a.kv_heads));
+    id /= (int64_t)a.n * a.kv_heads;
+    const int split = (int)(id % a.nsplit), tile = (int)(id / a.nsplit);
+    const int b = bh / a.kv_heads, h = bh % a.kv_heads;
+    const int len = keys_of(a, b), row0 = tile * 16 * NQ;
+
+    // this tile's keys: all of them, or in a causal call what its last row sees
+    int last_key = len;
+    if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + 16 * NQ - 1, a.rows - 1) / a.group + 1));
+    const int chunks = (last_key + 31) / 32, share = (chunks + a.nsplit - 1) / a.nsplit;
+    const int chunk0 = split * share, chunk1 = min(chunks, chunk0 + share);
+
+    // q in the second operand's layout: lane x16 holds row x16, lane group g its quarter of the row
+    u32x4 qf[NQ][F::QTERMS][F::MATH32 ? DP / 16 : DP / 32];
+    int lim[NQ];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        const int r = row0 + 16 * t + x16, rc = min(r, a.rows - 1);
+        lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
+        const char* qp = a.q + (int64_t)b * a.q_stride[0] + (int64_t)(rc / a.group) * a.q_stride[1] + (int64_t)(h * a.group + rc % a.group) * a.q_stride[2];
+        if constexpr (F::MATH32) {
+#pragma unroll
+            for (int u = 0; u < DP / 16; ++u) {
+                const int at = quarter_at<KVT>(g, 4 * u);
+                qf[t][0][u] = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 4 * at) : u32x4{};
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < DP / 32; ++u) {
+                const int at = quarter_at<KVT>(g, 8 * u);                  // eight consecutive values
+                const bool in = at < a.d && r < a.rows;
+                if constexpr (F::QTERMS == 1) qf[t][0][u] = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
+                else {
+                    float x[8];
+                    if constexpr (QT == ASR_F32) {
+                        const f32x4 p = in ? *reinterpret_cast<const f32x4*>(qp + 4 * at) : f32x4{};
+                        const f32x4 p2 = in ? *reinterpret_cast<const f32x4*>(qp + 4 * at + 16) : f32x4{};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { x[j] = p[j]; x[4 + j] = p2[j]; }
+                    } else {
+                        const u32x4 p = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { const f32x2 y = unpack16<true>(p[j]); x[2 * j] = y[0]; x[2 * j + 1] = y[1]; }
+                    }
+#pragma unroll
+                    for (int term = 0; term < F::QTERMS; ++term)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t w = pack_bf16(x[2 * j], x[2 * j + 1]);
+                            qf[t][term][u][j] = w;
+                            const f32x2 y = unpack16<false>(w);
+                            // an infinite value has no rest (inf - inf would make NaN of it)
+                            x[2 * j] = __builtin_isinf(y[0]) ? 0.0f : x[2 * j] - y[0];
+                            x[2 * j + 1] = __builtin_isinf(y[1]) ? 0.0f : x[2 * j + 1] - y[1];
+                        }
+                }
+            }
+        }
+    }
+
+    f32x4 o[NQ][F::NO];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        m[t] = NEG_INF;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < F::NO; ++i) o[t][i] = f32x4{};
+    }
+    const char* kb = a.k + (int64_t)b * a.k_stride[0] + (int64_t)h * a.k_stride[2];
+    const char* vb = a.v + (int64_t)b * a.v_stride[0] + (int64_t)h * a.v_stride[2];
+    const float *ksc = nullptr, *vsc = nullptr;
+    if constexpr (F::CODES) {
+        ksc = a.k_scale + (int64_t)bh * a.scale_stride;
+        vsc = a.v_scale + (int64_t)bh * a.scale_stride;
+    }
+    const bool full = a.d == DP;
+
+    for (int chunk = chunk0 + wave; chunk < chunk1; chunk += FEW_WAVES) {
+        const int c0 = chunk * 32;
+        // one admitted-bit per key of the chunk, the same for the whole wave
+        const int mk = c0 + (lane & 31);
+        const bool ok = mk < len && (!a.pad || a.pad[(int64_t)b * a.pad_stride + mk] == 0);
+        const uint32_t mask = (uint32_t)__ballot(ok);
+        if (mask == 0) continue;
+        const uint32_t mine = mask >> (8 * g);                                 // bits 0 .. 7: keys 8 g .. 8 g + 7
+
+        // K: tile t2's row x16 is key 8 (x16 / 4) + 4 t2 + x16 % 4; V: lane group g has keys 8 g .. 8 g + 7, lane x16 a sixteenth of each row.
+        // Keys past the end are read from the last one.
+        uint32_t kr[2][F::KW], vr[8][F::VW];
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            const int key = min(c0 + 8 * (x16 >> 2) + 4 * t2 + (x16 & 3), len - 1);
+            const char* p = kb + (uint64_t)(uint32_t)key * (uint64_t)a.k_stride[1];
+#pragma unroll
+            for (int w = 0; w < F::KW; w += 4) {
+                const int at = quarter_at<KVT>(g, w * 4 / F::KVB);
+                const u32x4 x = *reinterpret_cast<const u32x4*>(p + (full || at < a.d ? at * F::KVB : 0));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) kr[t2][w + j] = full || at < a.d ? x[j] : 0u;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = min(c0 + 8 * g + j, len - 1);
+            const char* p = vb + (uint64_t)(uint32_t)key * (uint64_t)a.v_stride[1];
+            if constexpr (F::MATH32) {
+#pragma unroll
+                for (int u = 0; u < DP / 64; ++u) {
+                    const int at = 64 * u + 4 * x16;
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(p + (full || at < a.d ? at * 4 : 0));
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vr[j][4 * u + w] = x[w];
+                }
+            } else {
+                const int at = DP / 16 * x16;
+                p += full || at < a.d ? at * F::KVB : 0;
+                if constexpr (F::VW == 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vr[j][w] = x[w];
+                } else if constexpr (F::VW == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+                    vr[j][0] = x[0];
+                    vr[j][1] = x[1];
+                } else vr[j][0] = *reinterpret_cast<const uint32_t*>(p);
+            }
+        }
+        if (mask != 0xffffffffu) {                                             // what is not admitted may hold anything: P = 0 meets V = 0
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int w = 0; w < F::VW; ++w) vr[j][w] = (mine >> j) & 1 ? vr[j][w] : 0u;
+        }
+        float ks = 1.0f, vs = 1.0f;
+        if constexpr (F::CODES) {
+            ks = ksc[c0 / ASR_KV8_BLOCK];
+            vs = vsc[c0 / ASR_KV8_BLOCK];
+        }
+
+        // S^T
+        f32x4 s[NQ][2];
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) s[t][0] = s[t][1] = f32x4{};
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            if constexpr (F::MATH32) {
+#pragma unroll
+                for (int w = 0; w < F::KW; ++w)
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t)
+                        s[t][t2] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t2][w]), __uint_as_float(qf[t][0][w / 4][w % 4]), s[t][t2], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int u = 0; u < DP / 32; ++u) {
+                    u32x4 kf;
+                    if constexpr (F::CODES) {
+                        kf[0] = codes_bf16<false>(kr[t2][2 * u], ks);
+                        kf[1] = codes_bf16<true>(kr[t2][2 * u], ks);
+                        kf[2] = codes_bf16<false>(kr[t2][2 * u + 1], ks);
+                        kf[3] = codes_bf16<true>(kr[t2][2 * u + 1], ks);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) kf[j] = kr[t2][4 * u + j];
+                    }
+#pragma unroll
+                    for (int term = F::QTERMS - 1; term >= 0; --term)
+#pragma unroll
+                        for (int t = 0; t < NQ; ++t) s[t][t2] = mfma16<F::F16>(kf, qf[t][term][u], s[t][t2]);
+                }
+            }
+        }
+
+        // soft-max step; p[t][4 t2 + i] belongs to key 8 g + 4 t2 + i
+        float p[NQ][8];
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[t][j] = s[t][j >> 2][j & 3] * a.c;
+            if (mask != 0xffffffffu || a.causal) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[t][j] = ((mine >> j) & 1) && c0 + 8 * g + j < lim[t] ? p[t][j] : NEG_INF;
+            }
+            float top = p[t][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, p[t][j]);
+            top = fmaxf(m[t], groups_max(top));
+            const float f = rescale(m[t], top), base = top == NEG_INF ? 0.0f : top;
+            m[t] = top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[t][j] = __builtin_amdgcn_exp2f(p[t][j] - base);
+                sum += p[t][j];
+            }
+            l[t] = l[t] * f + sum;
+#pragma unroll
+            for (int i = 0; i < F::NO; ++i) o[t][i] *= f;
+        }
+
+        // O^T += V^T P^T
+        if constexpr (F::MATH32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int w = 0; w < F::VW; ++w)
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t) o[t][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][w]), p[t][j], o[t][w], 0, 0, 0);
+        } else {
+            u32x4 pf[NQ][F::PTERMS];
+#pragma unroll
+            for (int t = 0; t < NQ; ++t)
+#pragma unroll
+                for (int term = 0; term < F::PTERMS; ++term)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t w = pack16<F::F16>(p[t][2 * j], p[t][2 * j + 1]);
+                        pf[t][term][j] = w;
+                        const f32x2 y = unpack16<F::F16>(w);
+                        p[t][2 * j] -= y[0];
+                        p[t][2 * j + 1] -= y[1];
+                    }
+#pragma unroll
+            for (int i = 0; i < F::NO; ++i) {
+                u32x4 vf;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (F::CODES) {
+                        const uint32_t two = __builtin_amdgcn_perm(vr[2 * j + 1][i >> 2], vr[2 * j][i >> 2], i & 2 ? 0x07030602u : 0x05010400u);
+                        vf[j] = i & 1 ? codes_bf16<true>(two, vs) : codes_bf16<false>(two, vs);
+                    } else {
+                        vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][i >> 1], vr[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                }
+#pragma unroll
+                for (int term = F::PTERMS - 1; term >= 0; --term)
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t) o[t][i] = mfma16<F::F16>(vf, pf[t][term], o[t][i]);
+            }
+        }
+    }
+
+    // join the waves
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+        const float sum = groups_sum(l[t]);
+        if (g == 0) {
+            s_m[wave][16 * t + x16] = m[t];
+            s_l[wave][16 * t + x16] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < F::NO; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = F::MATH32 ? 64 * (i >> 2) + 4 * (4 * g + j) + (i & 3) : DP / 16 * (4 * g + j) + i;
+                s_o[wave][16 * t + x16][at] = o[t][i][j];
+            }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * NQ * (DP / 4); e += 64 * FEW_WAVES) {
+        const int rr = e / (DP / 4), at = e % (DP / 4) * 4, r = row0 + rr;
+        if (r >= a.rows || at >= a.d) continue;
+        float top = s_m[0][rr];
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; ++w) top = fmaxf(top, s_m[w][rr]);
+        float sum = 0.0f;
+        f32x4 acc{};
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) {
+            const float f = rescale(s_m[w][rr], top);
+            sum += s_l[w][rr] * f;
+            acc += *reinterpret_cast<const f32x4*>(&s_o[w][rr][at]) * f;
+        }
+        if (a.nsplit > 1) {
+            float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
+            if (at == 0) { ws[0] = top; ws[1] = sum; }
+            *reinterpret_cast<f32x4*>(ws + 4 + at) = acc;
+        } else {
+            acc = sum == 0.0f ? f32x4{} : acc * (1.0f / sum);
+            char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] +
+                       (int64_t)(h * a.group + r % a.group) * a.out_stride[2] + at * F::QB;
+            if constexpr (QT == ASR_F32) *reinterpret_cast<f32x4*>(op) = acc;
+            else {
+                u32x2 w;
+                w[0] = pack16<QT == ASR_F16>(acc[0], acc[1]);
+                w[1] = pack16<QT == ASR_F16>(acc[2], acc[3]);
+                *reinterpret_cast<u32x2*>(op) = w;
+            }
+        }
+    }
+}
+
+// joins the shares of a long key axis: one thread per four output values
+template <int QT> __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a)
+{
+    const int per_row = a.d / 4;
+    const int64_t total = (int64_t)a.n * a.kv_heads * a.rows * per_row;
+    const int64_t split_stride = (int64_t)a.n * a.kv_heads * a.rows * (a.d + 4);
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        const int at = (int)(e % per_row) * 4;
+        const int64_t row = e / per_row;
+        const int r = (int)(row % a.rows), bh = (int)(row / a.rows), b = bh / a.kv_heads, h = bh % a.kv_heads;
+        const float* ws = a.ws + row * (a.d + 4);
+        float top = NEG_INF;
+        for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, ws[s * split_stride]);
+        float sum = 0.0f;
+        f32x4 acc{};
+        for (int s = 0; s < a.nsplit; ++s) {
+            const float* p = ws + s * split_stride;
+            const float f = rescale(p[0], top);
+            sum += p[1] * f;
+            acc += *reinterpret_cast<const f32x4*>(p + 4 + at) * f;
+        }
+        acc = sum == 0.0f ? f32x4{} : acc * (1.0f / sum);
+        char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] +
+                   (int64_t)(h * a.group + r % a.group) * a.out_stride[2] + at * (QT == ASR_F32 ? 4 : 2);
+        if constexpr (QT == ASR_F32) *reinterpret_cast<f32x4*>(op) = acc;
+        else {
+            u32x2 w;
+            w[0] = pack16<QT == ASR_F16>(acc[0], acc[1]);
+            w[1] = pack16<QT == ASR_F16>(acc[2], acc[3]);
+            *reinterpret_cast<u32x2*>(op) = w;
+        }
+    }
+}
+
+// ---- the choice of kernel -----------------------------------------------------------------------------------------------
+struct Plan {
+    int rows, tiles, nq, nsplit;
+    int64_t ws_bytes;
+};
+
+Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d)
+{
+    Plan p{};
+    p.rows = (int)(tq * (heads / kv_heads));
+    p.nq = p.rows > 16 ? 2 : 1;
+    p.tiles = (p.rows + 16 * p.nq - 1) / (16 * p.nq);
+    // shares of the key axis: enough workgroups for the chip (two for each of 256 compute units), each with at least four chunks of 32 keys for each wave
+    const int64_t wgs = n * kv_heads * p.tiles, most = tk / (FEW_WAVES * 32 * 4);
+    int64_t split = wgs > 0 ? (512 + wgs - 1) / wgs : 1;
+    if (split > most) split = most;
+    if (split > 64) split = 64;
+    p.nsplit = split < 1 ? 1 : (int)split;
+    p.ws_bytes = p.nsplit > 1 ? (int64_t)p.nsplit * n * kv_heads * p.rows * (d + 4) * 4 : 0;
+    return p;
+}
+
+template <int QT, int KVT> hipError_t launch_few(const AttnArgs& a, int nq, hipStream_t s)
+{
+    const dim3 grid((uint32_t)((int64_t)a.n * a.kv_heads * a.nsplit * a.tiles)), block(64 * FEW_WAVES);
+    if (a.d <= 64) return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 64, 1>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 64, 2>, grid, block, s, a);
+    return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 128, 1>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 128, 2>, grid, block, s, a);
+}
+
+template <int QT> hipError_t launch_join(const AttnArgs& a, hipStream_t s)
+{
+    const int64_t blocks = ((int64_t)a.n * a.kv_heads * a.rows * (a.d / 4) + 255) / 256;
+    return ops_launch(attention_join_kernel<QT>, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), s, a);
+}
+
+template <int QT, int KVT> int attend(const char* what, AttnArgs& a, const Plan& p, void* ws, int64_t ws_bytes, hipStream_t s)
+{
+    a.rows = p.rows;
+    a.tiles = p.tiles;
+    a.nsplit = p.nsplit;
+    if (p.ws_bytes > 0) {
+        if (!ws || ws_bytes < p.ws_bytes) return ops_fail(ASR_ERR_CAPACITY, "%s: the workspace must hold %lld bytes", what, (long long)p.ws_bytes);
+        if (reinterpret_cast<uintptr_t>(ws) & 15) return ops_fail(ASR_ERR_ARG, "%s: the workspace must be 16-byte aligned", what);
+        a.ws = static_cast<float*>(ws);
+    }
+    hipError_t e = launch_few<QT, KVT>(a, p.nq, s);
+    if (e == hipSuccess && p.nsplit > 1) e = launch_join<QT>(a, s);
+    return ops_launched(what, e);
+}
+
+// what both operators ask of their sizes; null: fine
+const char* bad_sizes(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, int64_t d_step)
+{
+    if (n < 0 || tq < 0 || tk < 0) return "negative sizes";
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads) return "heads must be a multiple of kv_heads";
+    if (d < d_step || d > 128 || d % d_step) return d_step == 8 ? "d must be a multiple of 8 in 8..128" : "d must be a multiple of 16 in 16..128";
+    if (tk > 0x7fffffff - 64 || tq * heads > 0x7fffffff / 2) return "too many query rows or keys";
+    const int64_t rows = tq * (heads / kv_heads);
+    // workgroups of 256 threads in one grid dimension, whatever the split
+    if (n * kv_heads > (1 << 22) || n * kv_heads * ((rows + 15) / 16) > (1 << 22)) return "too many sequences, heads and query rows for one call";
+    return nullptr;
+}
+
+bool nonnegative(const int64_t* s) { return s[0] >= 0 && s[1] >= 0 && s[2] >= 0; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t asr_cross_attention_workspace(int32_t n, int32_t tq, int32_t tk, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype)
+{
+    if (bad_sizes(n, tq, tk, heads, kv_heads, d, 8) || !ops_dtype_ok(dtype)) return 0;
+    return plan_of(n, tq, tk, heads, kv_heads, d).ws_bytes;
+}
+
+int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
+{
+    if (!a) return ops_fail(ASR_ERR_ARG, "null argument");
+    if (const char* why = bad_sizes(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d, 8)) return ops_fail(ASR_ERR_ARG, "cross_attention: %s", why);
+    if (!ops_dtype_ok(a->dtype)) return ops_fail(ASR_ERR_ARG, "cross_attention: unknown dtype %d", a->dtype);
+    if (!isfinite(a->scale)) return ops_fail(ASR_ERR_ARG, "cross_attention: the scale must be finite");
+    if (a->n == 0 || a->tq == 0) return ASR_OK;
+    if (!a->q || !a->out || (a->tk > 0 && (!a->k || !a->v))) return ops_fail(ASR_ERR_ARG, "cross_attention: null argument");
+    if (!nonnegative(a->q_stride) || !nonnegative(a->k_stride) || !nonnegative(a->v_stride) || !nonnegative(a->out_stride) || a->pad_stride < 0)
+        return ops_fail(ASR_ERR_ARG, "cross_attention: negative stride");
+    if (!ops_rows16(a->q, a->q_stride, a->n, a->tq, a->heads, a->dtype) || !ops_rows16(a->out, a->out_stride, a->n, a->tq, a->heads, a->dtype) ||
+        (a->tk > 0 && (!ops_rows16(a->k, a->k_stride, a->n, a->tk, a->kv_heads, a->dtype) ||
+                       !ops_rows16(a->v, a->v_stride, a->n, a->tk, a->kv_heads, a->dtype))))
+        return ops_fail(ASR_ERR_ARG, "cross_attention: every row of q, k, v and out must start on 16 bytes");
+    AttnArgs x{};
+    const int64_t size = ops_dtype_size(a->dtype);
+    x.q = static_cast<const char*>(a->q); x.k = static_cast<const char*>(a->k); x.v = static_cast<const char*>(a->v);
+    x.out = static_cast<char*>(a->out);
+    x.lens = a->lens; x.pad = a->pad; x.pad_stride = a->pad_stride;
+    for (int i = 0; i < 3; ++i) {
+        x.q_stride[i] = a->q_stride[i] * size; x.out_stride[i] = a->out_stride[i] * size;
+        x.k_stride[i] = a->k_stride[i] * size; x.v_stride[i] = a->v_stride[i] * size;
+    }
+    x.n = a->n; x.tq = a->tq; x.tk = a->tk; x.kv_heads = a->kv_heads; x.group = a->heads / a->kv_heads; x.d = a->d;
+    x.c = a->scale * LOG2E;
+    const Plan p = plan_of(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a->dtype == ASR_F32) return attend<ASR_F32, KV_F32>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
+    if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_BF16>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
+    return attend<ASR_F16, KV_F16>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
+}
+
+int64_t asr_kv8_attention_workspace(int32_t n, int32_t tq, int32_t capacity, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype)
+{
+    if (bad_sizes(n, tq, capacity, heads, kv_heads, d, 16) || !ops_dtype_ok(dtype)) return 0;
+    return plan_of(n, tq, capacity, heads, kv_heads, d).ws_bytes;
+}
+
+int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
+{
+    if (!a) return ops_fail(ASR_ERR_ARG, "null argument");
+    if (const char* why = bad_sizes(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d, 16)) return ops_fail(ASR_ERR_ARG, "kv8_attention: %s", why);
+    if (a->capacity % ASR_KV8_BLOCK) return ops_fail(ASR_ERR_ARG, "kv8_attention: the capacity must be a multiple of %d tokens", ASR_KV8_BLOCK);
+    if (!ops_dtype_ok(a->dtype)) return ops_fail(ASR_ERR_ARG, "kv8_attention: unknown dtype %d", a->dtype);
+    if (!isfinite(a->scale)) return ops_fail(ASR_ERR_ARG, "kv8_attention: the scale must be finite");
+    if (a->n == 0 || a->tq == 0) return ASR_OK;
+    if (!a->q || !a->out || !a->lens || (a->capacity > 0 && (!a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale)))
+        return ops_fail(ASR_ERR_ARG, "kv8_attention: null argument");
+    if (!nonnegative(a->q_stride) || !nonnegative(a->out_stride) || a->cache_stride[0] < 0 || a->cache_stride[1] < 0)
+        return ops_fail(ASR_ERR_ARG, "kv8_attention: negative stride");
+    if (!ops_rows16(a->q, a->q_stride, a->n, a->tq, a->heads, a->dtype) || !ops_rows16(a->out, a->out_stride, a->n, a->tq, a->heads, a->dtype))
+        return ops_fail(ASR_ERR_ARG, "kv8_attention: every row of q and out must start on 16 bytes");
+    if (((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) || a->cache_stride[0] % 16 || a->cache_stride[1] % 16)
+        return ops_fail(ASR_ERR_ARG, "kv8_attention: cache rows must start on 16 bytes");
+    AttnArgs x{};
+    const int64_t size = ops_dtype_size(a->dtype);
+    x.q = static_cast<const char*>(a->q); x.out = static_cast<char*>(a->out);
+    x.k = reinterpret_cast<const char*>(a->k_cache); x.v = reinterpret_cast<const char*>(a->v_cache);
+    x.k_scale = a->k_scale; x.v_scale = a->v_scale; x.scale_stride = a->capacity / ASR_KV8_BLOCK;
+    x.lens = a->lens;
+    for (int i = 0; i < 3; ++i) { x.q_stride[i] = a->q_stride[i] * size; x.out_stride[i] = a->out_stride[i] * size; }
+    x.k_stride[0] = x.v_stride[0] = a->cache_stride[0];
+    x.k_stride[1] = x.v_stride[1] = a->d;
+    x.k_stride[2] = x.v_stride[2] = a->cache_stride[1];
+    x.n = a->n; x.tq = a->tq; x.tk = a->capacity; x.kv_heads = a->kv_heads; x.group = a->heads / a->kv_heads; x.d = a->d;
+    x.causal = a->causal ? 1 : 0;
+    x.c = a->scale * LOG2E;
+    const Plan p = plan_of(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a->dtype == ASR_F32) return attend<ASR_F32, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
+    if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
+    return attend<ASR_F16, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
+}
+
+}  // extern "C"

@@ -269,6 +269,112 @@ int asr_op_beam_step(asr_handle* h, const float* scores, const int32_t* finished
                      const float* cand_scores, const int32_t* cand_tokens, int32_t b, int32_t k,
                      float* new_scores, int32_t* tokens, int32_t* parents, int32_t* finished_out);
 
+/* ---- operators on device memory ---------------------------------------------------------------
+ * What scoring and serving code needs beside the engine, on the caller's own device arrays and stream: the log probabilities of given
+ * tokens, attention over encoder states of another length, and attention over K/V caches held in 8 bits.  They need no handle.
+ * Unlike the entry points above they do NOT block: the work is queued on `stream` (a hipStream_t; 0 = the default stream) of the
+ * CURRENT device, which has to be the one that holds the arrays, and can be captured into a HIP graph.  Nothing is allocated and nothing
+ * is kept between calls; the workspace of a call is the caller's and must not be shared by calls that may run at the same time.
+ * Every argument struct starts as zero bytes; pointers are device pointers; strides count ELEMENTS of the array's type.  On a status other than ASR_OK
+ * nothing was queued and asr_ops_last_error() (per host thread) says why.  asr_amd/ops.py is the Python form on torch tensors. */
+
+enum asr_dtype { ASR_F32 = 0, ASR_BF16 = 1, ASR_F16 = 2 };
+
+const char* asr_ops_last_error(void);
+
+/* Per row of logits [rows, vocab] (row r at logits + r * row_stride, vocabulary contiguous): with p = softmax(row),
+ *   logprob[r] = log p(tokens[r]),  entropy[r] = - sum_v p_v log p_v,
+ *   top_tokens[r, 0..top) = the `top` tokens of the largest logits in descending order, ties to the lower token, top_logprobs = their log p.
+ * A negative token stands for "no token" (padding): its log probability is 0.  A token >= vocab gives NaN.  Logits of -infinity
+ * are masked-out tokens (p = 0, no share in the entropy); a row with nothing else gives log p = -infinity and entropy 0.  A row with a NaN or
+ * +infinity gives NaN throughout (its top_tokens are valid token numbers, no more).
+ * Everything is computed in float32.  model.py:345-360 has the pieces: log_softmax + top_k of test_output, the cross entropy of test_loss. */
+typedef struct asr_token_logprobs_args {
+    const void* logits;
+    const void* tokens;                  /* [rows] int32 or int64 */
+    float* logprob;                      /* [rows] */
+    float* entropy;                      /* [rows] */
+    float* top_logprobs;                 /* [rows, top]; may be null when top is 0 */
+    int32_t* top_tokens;                 /* [rows, top]; may be null when top is 0 */
+    int64_t rows, row_stride;
+    int32_t vocab;                       /* 1 .. 2^30 */
+    int32_t top;                         /* 0 .. min(32, vocab) */
+    int32_t dtype;                       /* enum asr_dtype of the logits */
+    int32_t token_bytes;                 /* 4 or 8 */
+} asr_token_logprobs_args;
+int asr_token_logprobs(const asr_token_logprobs_args* a, void* stream);
+
+/* Attention of many or few query rows over the states of another sequence (utils.py:609-631 with encdec keys):
+ *   out[b, i, h] = softmax_j(scale * q[b, i, h] . k[b, j, h / (heads / kv_heads)]) v[b, j, ...]  over the admitted j,
+ * admitted: j < lens[b] (lens null: all tk; values are taken as 0 below 0 and as tk above tk) and pad[b, j] == 0 (pad null: no flags).  What
+ * stands in positions that are not admitted does not matter, NaN and infinity included; a query without an admitted position gives 0.  Beams
+ * of one utterance are query rows (tq = beams): nothing orders the queries.
+ * q, out: [n, tq, heads, d], k, v: [n, tk, kv_heads, d] of one type (bf16 and f16 are multiplied on the 16-bit matrix instruction, f32 on the
+ * exact float32 one; scores, soft-max statistics and sums are float32), d contiguous, every other stride free but such that each row starts on
+ * 16 bytes; out may not overlap the inputs.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
+typedef struct asr_cross_attention_args {
+    const void *q, *k, *v;
+    void* out;
+    const int32_t* lens;                 /* [n] or null */
+    const uint8_t* pad;                  /* [n, tk] bytes, row b at pad + b * pad_stride, or null */
+    void* workspace;                     /* asr_cross_attention_workspace() bytes, 16-byte aligned (null if that is 0) */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];        /* of n, t and head */
+    int64_t pad_stride;
+    int64_t workspace_bytes;
+    int32_t n, tq, tk, heads, kv_heads, d;
+    int32_t dtype;                       /* enum asr_dtype */
+    float scale;
+} asr_cross_attention_args;
+int64_t asr_cross_attention_workspace(int32_t n, int32_t tq, int32_t tk, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype);
+int asr_cross_attention(const asr_cross_attention_args* a, void* stream);
+
+/* The 8-bit K/V cache: codes [n, kv_heads, capacity, d] in OCP e4m3 and one float32 scale, a power of two, for every block of
+ * ASR_KV8_BLOCK tokens and head, [n, kv_heads, capacity / ASR_KV8_BLOCK]; a value is code * scale.  K and V have codes and scales of their own.
+ * Codes lie such that tokens of one (sequence, head) are d bytes apart; scales are dense. */
+#define ASR_KV8_BLOCK 64
+
+/* Writes tokens lens[b] .. lens[b] + counts[b] of every sequence b (counts null: all `new_tokens`; tokens past the capacity are dropped, a
+ * sequence with lens[b] < 0 or counts[b] <= 0 is left alone).  The scale of a block is the smallest power of two, 2^-100 at the least, with which
+ * every finite magnitude it was made for stays within 448, the largest e4m3 value; a value is rounded once, to the nearest code, halves to
+ * even.  A block that held tokens before (lens[b] inside it) keeps its scale or takes the larger one its new tokens need; its older tokens are then
+ * coded again under it.  Infinities are held as +-448, NaN stays NaN; neither counts for a scale.  Nothing else is written: blocks
+ * without new tokens, and positions behind the last one, stay as they are.  No two sequences may share cache memory.
+ * k, v: [n, new_tokens, kv_heads, d], any asr_dtype, rows on 16 bytes.  d % 16 == 0, 16 <= d <= 128; capacity % ASR_KV8_BLOCK == 0. */
+typedef struct asr_kv8_append_args {
+    const void *k, *v;
+    uint8_t *k_cache, *v_cache;          /* codes of sequence b, head h at + b * cache_stride[0] + h * cache_stride[1] */
+    float *k_scale, *v_scale;
+    const int32_t* lens;                 /* [n] tokens held before this call */
+    const int32_t* counts;               /* [n] new tokens, or null */
+    int64_t k_stride[3], v_stride[3];    /* of n, t and head */
+    int64_t cache_stride[2];             /* both caches */
+    int32_t n, new_tokens, kv_heads, d, capacity;
+    int32_t dtype;                       /* enum asr_dtype of k and v */
+} asr_kv8_append_args;
+int asr_kv8_append(const asr_kv8_append_args* a, void* stream);
+
+/* asr_cross_attention with the cache above for keys and values; lens[b] tokens are valid (taken as 0 below 0, as the capacity above it).
+ * causal: query i of sequence b is its token lens[b] - tq + i and sees nothing behind itself (the cache already holds the tq newest tokens; a
+ * query with nothing to see gives 0).  Codes are multiplied exactly on the 16-bit matrix instruction; a q of f16 or f32 enters as
+ * two or three bf16 terms, so nothing of it is lost. */
+typedef struct asr_kv8_attention_args {
+    const void* q;
+    void* out;
+    const uint8_t *k_cache, *v_cache;
+    const float *k_scale, *v_scale;
+    const int32_t* lens;                 /* [n] */
+    void* workspace;                     /* asr_kv8_attention_workspace() bytes, 16-byte aligned (null if that is 0) */
+    int64_t q_stride[3], out_stride[3];  /* of n, t and head */
+    int64_t cache_stride[2];             /* of n and head, both caches */
+    int64_t workspace_bytes;
+    int32_t n, tq, heads, kv_heads, d, capacity;
+    int32_t dtype;                       /* enum asr_dtype of q and out */
+    int32_t causal;
+    float scale;
+} asr_kv8_attention_args;
+int64_t asr_kv8_attention_workspace(int32_t n, int32_t tq, int32_t capacity, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype);
+int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream);
+
 /* ---- instrumentation ---------------------------------------------------------------------- */
 
 /* mode 0: normal.  mode 1: bracket every kernel launch of subsequent calls with HIP events on the
