@@ -40,8 +40,10 @@ namespace {
 // strip (rescaled when the maximum of a group of loads beats m), the workgroup joins them, and
 //     log p(t) = x_t - m - ln S,      H = ln S - T / S
 // (both terms of H are >= 0: nothing cancels).  The difference x - m is taken before the factor log2(e), so that large logits lose nothing.
-// The alternatives come without a second pass over the row: the k-th largest of the threads' maxima is a bound that at least k logits reach, and only
-// the threads whose own maximum reaches it read their strip again and collect what does (usually k to 2k values).
+// The alternatives come without a second pass over the row: the strips' maxima are joined to 64 groups', a bound that the maxima of at least `top` and
+// hardly more groups reach is found by bisection over them (one wave, a ballot a step); only the strips whose own maximum reaches it are read again
+// (by the whole workgroup, from the cache), what reaches the bound is collected (usually little more than `top` values) and ranked.  Where that does not fit the list - masked rows of fewer than `top` admitted
+// tokens, equal logits, the likeliest tokens all in a few strips - the alternatives are taken one by one instead.
 
 __device__ inline float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ inline float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -50,6 +52,7 @@ template <int DT> struct Elem;
 template <> struct Elem<ASR_F32> {
     typedef float T;
     static constexpr int PER = 4;
+    static constexpr uint32_t NONE = 0xff800000u;              // -infinity in every place of a word
     static __device__ float one(const float* p) { return *p; }
     static __device__ void unpack(const u32x4& r, float* x)
     {
@@ -60,6 +63,7 @@ template <> struct Elem<ASR_F32> {
 template <> struct Elem<ASR_BF16> {
     typedef uint16_t T;
     static constexpr int PER = 8;
+    static constexpr uint32_t NONE = 0xff80ff80u;
     static __device__ float one(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
     static __device__ void unpack(const u32x4& r, float* x)
     {
@@ -70,6 +74,7 @@ template <> struct Elem<ASR_BF16> {
 template <> struct Elem<ASR_F16> {
     typedef _Float16 T;
     static constexpr int PER = 8;
+    static constexpr uint32_t NONE = 0xfc00fc00u;
     static __device__ float one(const _Float16* p) { return (float)*p; }
     static __device__ void unpack(const u32x4& r, float* x)
     {
@@ -109,12 +114,29 @@ __device__ inline Stats at_max(const Stats& a, float m)
     r.t = a.m == NEG_INF ? f : (a.t + a.s * d) * f;
     return r;
 }
-__device__ inline Stats join(const Stats& a, const Stats& b)
+
+// maximum / sum over a wave: rotations inside rows of 16 lanes, then the rows
+template <int CTRL> __device__ inline float rotated(float x)
 {
-    const float m = fmaxf(a.m, b.m);
-    const Stats x = at_max(a, m), y = at_max(b, m);
-    return {m, x.s + y.s, x.t + y.t};
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
 }
+template <typename F> __device__ inline float row_reduce(float x, F f)
+{
+    x = f(x, rotated<0x128>(x));
+    x = f(x, rotated<0x124>(x));
+    x = f(x, rotated<0x122>(x));
+    return f(x, rotated<0x121>(x));
+}
+template <typename F> __device__ inline float wave_reduce(float x, F f)
+{
+    x = row_reduce(x, f);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Sum { __device__ float operator()(float a, float b) const { return a + b; } };
 
 template <int N> __device__ inline void add_group(Stats& st, const float* x)
 {
@@ -168,6 +190,7 @@ struct TokenLogprobsArgs {
 };
 
 constexpr int MAX_TOP = 32;
+constexpr int MAX_CANDIDATES = 512;
 constexpr int MAX_GRID = 1 << 20;        // workgroups; further rows are taken in turn
 
 template <int DT, int NT> __global__ __launch_bounds__(NT) void token_logprobs_kernel(TokenLogprobsArgs a)
@@ -175,79 +198,131 @@ template <int DT, int NT> __global__ __launch_bounds__(NT) void token_logprobs_k
     typedef typename Elem<DT>::T T;
     constexpr int PER = Elem<DT>::PER, NW = NT / 64, UNROLL = 4;
     __shared__ float red[3][NW];
-    __shared__ uint64_t wkey[NW];
+    __shared__ uint64_t wkey[NW], cand[MAX_CANDIDATES];
+    constexpr int GS = NT / 64;                                          // threads of a group; 64 groups
+    __shared__ uint32_t group_max[64], bound;
+    __shared__ uint16_t strips[NT];
+    __shared__ int n_strips, n_cand;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
         const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
         const int chunks = (a.vocab - head) / PER, body = head + chunks * PER;
+        // asked for first: the token's own logit and what lies outside the 16-byte chunks
+        const int64_t token = a.token_bytes == 8 ? static_cast<const int64_t*>(a.tokens)[r] : (int64_t) static_cast<const int32_t*>(a.tokens)[r];
+        const bool in = token >= 0 && token < a.vocab;
+        const float x_token = Elem<DT>::one(row + (in ? token : 0));
+        float ends[2] = {NEG_INF, NEG_INF};
+        if (tid < head) ends[0] = Elem<DT>::one(row + tid);
+        if (tid < a.vocab - body) ends[1] = Elem<DT>::one(row + body + tid);
+        const u32x4* v = reinterpret_cast<const u32x4*>(row + head);
         Stats st{NEG_INF, 0.0f, 0.0f};
-        {
-            const u32x4* v = reinterpret_cast<const u32x4*>(row + head);
-            int c = tid;
-            for (; c + (UNROLL - 1) * NT < chunks; c += UNROLL * NT) {
-                u32x4 raw[UNROLL];
+        for (int c = tid; c < chunks; c += UNROLL * NT) {
+            u32x4 raw[UNROLL];
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) raw[u] = v[c + u * NT];
-                float x[UNROLL * PER];
-#pragma unroll
-                for (int u = 0; u < UNROLL; ++u) Elem<DT>::unpack(raw[u], x + u * PER);
-                add_group<UNROLL * PER>(st, x);
+            for (int u = 0; u < UNROLL; ++u) {
+                raw[u] = u32x4{Elem<DT>::NONE, Elem<DT>::NONE, Elem<DT>::NONE, Elem<DT>::NONE};
+                if (c + u * NT < chunks) raw[u] = v[c + u * NT];
             }
-            for (; c < chunks; c += NT) {
-                float x[PER];
-                Elem<DT>::unpack(v[c], x);
-                add_group<PER>(st, x);
-            }
-            float one;
-            if (tid < head) { one = Elem<DT>::one(row + tid); add_group<1>(st, &one); }
-            if (tid < a.vocab - body) { one = Elem<DT>::one(row + body + tid); add_group<1>(st, &one); }
-        }
-        Stats w = st;
+            float x[UNROLL * PER];
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            const Stats other{__shfl_xor(w.m, o, 64), __shfl_xor(w.s, o, 64), __shfl_xor(w.t, o, 64)};
-            w = join(w, other);
+            for (int u = 0; u < UNROLL; ++u) Elem<DT>::unpack(raw[u], x + u * PER);
+            add_group<UNROLL * PER>(st, x);
         }
+        add_group<2>(st, ends);
+        // the waves' sums under the waves' maxima, then the workgroup's
+        Stats w = at_max(st, wave_reduce(st.m, Max()));
+        w.s = wave_reduce(w.s, Sum());
+        w.t = wave_reduce(w.t, Sum());
         if (lane == 0) { red[0][wave] = w.m; red[1][wave] = w.s; red[2][wave] = w.t; }
-        __syncthreads();
-        Stats all{red[0][0], red[1][0], red[2][0]};
+        float gm = st.m;
 #pragma unroll
-        for (int i = 1; i < NW; ++i) all = join(all, Stats{red[0][i], red[1][i], red[2][i]});
+        for (int o = 1; o < GS; o *= 2) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
+        if (tid % GS == 0) group_max[tid / GS] = ordered(gm);
+        __syncthreads();
+        const int l16 = lane & 15;                                       // every 16 lanes join the (at most 16) waves' sums
+        w = l16 < NW ? Stats{red[0][l16], red[1][l16], red[2][l16]} : Stats{NEG_INF, 0.0f, 0.0f};
+        Stats all = at_max(w, row_reduce(w.m, Max()));
+        all.s = row_reduce(all.s, Sum());
+        all.t = row_reduce(all.t, Sum());
         const bool none = all.m == NEG_INF && all.s == 0.0f;             // every token is masked out
         const float m = base_of(all.m), log_s = logf(all.s);
         if (tid == 0) {
-            const int64_t t = a.token_bytes == 8 ? static_cast<const int64_t*>(a.tokens)[r] : (int64_t) static_cast<const int32_t*>(a.tokens)[r];
-            float lp;
-            if (t < 0) lp = 0.0f;
-            else if (t >= a.vocab) lp = __builtin_nanf("");
-            else lp = none ? NEG_INF : (Elem<DT>::one(row + t) - m) - log_s;
+            const float lp = token < 0 ? 0.0f : !in ? __builtin_nanf("") : none ? NEG_INF : (x_token - m) - log_s;
             a.logprob[r] = lp;
             a.entropy[r] = none ? 0.0f : log_s - all.t / all.s;
         }
         if (a.top > 0) {
-            // One alternative a round: the workgroup's largest key; its owner then looks for the next one of its strip.
-            uint64_t mine = 0;
-            for_strip<DT, NT>(row, a.vocab, head, tid, [&](float x, int i) { const uint64_t k = key_of(x, i); mine = k > mine ? k : mine; });
-            for (int j = 0; j < a.top; ++j) {
-                const uint64_t best = shfl_max_u64(mine);
-                if (lane == 0) wkey[wave] = best;
-                __syncthreads();
-                uint64_t win = wkey[0];
-#pragma unroll
-                for (int i = 1; i < NW; ++i) win = wkey[i] > win ? wkey[i] : win;
-                __syncthreads();
-                if (tid == 0) {
-                    a.top_tokens[r * a.top + j] = (int32_t) ~(uint32_t)win;
-                    a.top_logprobs[r * a.top + j] = none ? NEG_INF : (unordered((uint32_t)(win >> 32)) - m) - log_s;
+            if (wave == 0) {
+                const uint32_t mine = group_max[lane];
+                uint32_t thr = 0;
+                for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                    const int n = __popcll(__ballot(mine >= (thr | bit)));
+                    if (n >= a.top) {
+                        thr |= bit;
+                        if (n <= a.top + 2) break;
+                    }
                 }
-                if (mine == win && j + 1 < a.top) {
-                    uint64_t next = 0;
-                    for_strip<DT, NT>(row, a.vocab, head, tid, [&](float x, int i) {
-                        const uint64_t k = key_of(x, i);
-                        next = (k < win && k > next) ? k : next;
-                    });
-                    mine = next;
+                if (lane == 0) { bound = thr; n_strips = 0; n_cand = 0; }
+            }
+            __syncthreads();
+            const uint32_t thr = bound;
+            if (ordered(st.m) >= thr) strips[atomicAdd(&n_strips, 1)] = (uint16_t)tid;
+            __syncthreads();
+            const auto collect = [&](float x, int i) {
+                if (ordered(x) >= thr) {
+                    const int at = atomicAdd(&n_cand, 1);
+                    if (at < MAX_CANDIDATES) cand[at] = key_of(x, i);
+                }
+            };
+            const int per_strip = (chunks + NT - 1) / NT, total = n_strips * per_strip;
+            for (int i = tid; i < total; i += NT) {
+                const int c = strips[i / per_strip] + i % per_strip * NT;
+                if (c < chunks) {
+                    float x[PER];
+                    Elem<DT>::unpack(v[c], x);
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) collect(x[j], head + c * PER + j);
+                }
+            }
+            if (tid < head) collect(ends[0], tid);
+            if (tid < a.vocab - body) collect(ends[1], body + tid);
+            __syncthreads();
+            const int found = n_cand;
+            if (found <= MAX_CANDIDATES) {
+                for (int i = tid; i < found; i += NT) {
+                    const uint64_t key = cand[i];
+                    int rank = 0;
+                    for (int j = 0; j < found; ++j) rank += cand[j] > key;
+                    if (rank < a.top) {
+                        a.top_tokens[r * a.top + rank] = (int32_t) ~(uint32_t)key;
+                        a.top_logprobs[r * a.top + rank] = none ? NEG_INF : (unordered((uint32_t)(key >> 32)) - m) - log_s;
+                    }
+                }
+            } else {
+                // One alternative a round: the workgroup's largest key; its owner then looks for the next one of its strip.
+                uint64_t mine = 0;
+                for_strip<DT, NT>(row, a.vocab, head, tid, [&](float x, int i) { const uint64_t k = key_of(x, i); mine = k > mine ? k : mine; });
+                for (int j = 0; j < a.top; ++j) {
+                    const uint64_t best = shfl_max_u64(mine);
+                    if (lane == 0) wkey[wave] = best;
+                    __syncthreads();
+                    uint64_t win = wkey[0];
+#pragma unroll
+                    for (int i = 1; i < NW; ++i) win = wkey[i] > win ? wkey[i] : win;
+                    __syncthreads();
+                    if (tid == 0) {
+                        a.top_tokens[r * a.top + j] = (int32_t) ~(uint32_t)win;
+                        a.top_logprobs[r * a.top + j] = none ? NEG_INF : (unordered((uint32_t)(win >> 32)) - m) - log_s;
+                    }
+                    if (mine == win && j + 1 < a.top) {
+                        uint64_t next = 0;
+                        for_strip<DT, NT>(row, a.vocab, head, tid, [&](float x, int i) {
+                            const uint64_t k = key_of(x, i);
+                            next = (k < win && k > next) ? k : next;
+                        });
+                        mine = next;
+                    }
                 }
             }
         }
@@ -257,7 +332,11 @@ template <int DT, int NT> __global__ __launch_bounds__(NT) void token_logprobs_k
 
 template <int DT> hipError_t run_token_logprobs(const TokenLogprobsArgs& k, hipStream_t s)
 {
-    return ops_launch(token_logprobs_kernel<DT, 256>, dim3((uint32_t)(k.rows < MAX_GRID ? k.rows : MAX_GRID)), dim3(256), s, k);
+    const dim3 grid((uint32_t)(k.rows < MAX_GRID ? k.rows : MAX_GRID));
+    // Few long rows: a row's loads wait for one another, so more threads share it (64 x 28444 bf16: 9.2 us with 256 threads, 7.5 with 1024; with 1024
+    // rows 19 and 29: there the rows fill the chip, and a wider workgroup only has more to join)
+    if (k.rows <= 256 && k.vocab / Elem<DT>::PER >= 2048) return ops_launch(token_logprobs_kernel<DT, 1024>, grid, dim3(1024), s, k);
+    return ops_launch(token_logprobs_kernel<DT, 256>, grid, dim3(256), s, k);
 }
 
 }  // namespace
