@@ -154,6 +154,22 @@ template <int N> __device__ inline void add_group(Stats& st, const float* x)
     }
 }
 
+// chunks c, c + NT, ... (N of them, those below `chunks`) of a row: loaded together, then added
+template <int DT, int NT, int N> __device__ inline void add_chunks(Stats& st, const u32x4* v, int c, int chunks)
+{
+    constexpr int PER = Elem<DT>::PER;
+    u32x4 raw[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        raw[u] = u32x4{Elem<DT>::NONE, Elem<DT>::NONE, Elem<DT>::NONE, Elem<DT>::NONE};
+        if (c + u * NT < chunks) raw[u] = v[c + u * NT];
+    }
+    float x[N * PER];
+#pragma unroll
+    for (int u = 0; u < N; ++u) Elem<DT>::unpack(raw[u], x + u * PER);
+    add_group<N * PER>(st, x);
+}
+
 __device__ inline uint64_t shfl_max_u64(uint64_t v)
 {
 #pragma unroll
@@ -196,7 +212,7 @@ constexpr int MAX_GRID = 1 << 20;        // workgroups; further rows are taken i
 template <int DT, int NT> __global__ __launch_bounds__(NT) void token_logprobs_kernel(TokenLogprobsArgs a)
 {
     typedef typename Elem<DT>::T T;
-    constexpr int PER = Elem<DT>::PER, NW = NT / 64, UNROLL = 4;
+    constexpr int PER = Elem<DT>::PER, NW = NT / 64;
     __shared__ float red[3][NW];
     __shared__ uint64_t wkey[NW], cand[MAX_CANDIDATES];
     constexpr int GS = NT / 64;                                          // threads of a group; 64 groups
@@ -217,18 +233,10 @@ template <int DT, int NT> __global__ __launch_bounds__(NT) void token_logprobs_k
         if (tid < a.vocab - body) ends[1] = Elem<DT>::one(row + body + tid);
         const u32x4* v = reinterpret_cast<const u32x4*>(row + head);
         Stats st{NEG_INF, 0.0f, 0.0f};
-        for (int c = tid; c < chunks; c += UNROLL * NT) {
-            u32x4 raw[UNROLL];
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) {
-                raw[u] = u32x4{Elem<DT>::NONE, Elem<DT>::NONE, Elem<DT>::NONE, Elem<DT>::NONE};
-                if (c + u * NT < chunks) raw[u] = v[c + u * NT];
-            }
-            float x[UNROLL * PER];
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) Elem<DT>::unpack(raw[u], x + u * PER);
-            add_group<UNROLL * PER>(st, x);
-        }
+        int c0 = 0;
+        for (; chunks - c0 > 2 * NT; c0 += 4 * NT) add_chunks<DT, NT, 4>(st, v, c0 + tid, chunks);
+        if (chunks - c0 > NT) add_chunks<DT, NT, 2>(st, v, c0 + tid, chunks);
+        else if (chunks > c0) add_chunks<DT, NT, 1>(st, v, c0 + tid, chunks);
         add_group<2>(st, ends);
         // the waves' sums under the waves' maxima, then the workgroup's
         Stats w = at_max(st, wave_reduce(st.m, Max()));
