@@ -426,6 +426,248 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
     }
 }
 
+// ---- many rows: the waves of a workgroup share tiles of keys in LDS ------------------------------------------------------
+// 16-bit products only.  A workgroup has 128 rows, 32 for each of its four waves, and walks over tiles of 64 keys that it stages into LDS (two
+// buffers: the next tile's loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
+// scale).  32 x 32 x 16 products: S^T = K q^T has a row in each lane of 32 and lane half; O^T = V^T P^T takes V^T from LDS with the transposing read
+// (four keys of one column a lane) and P^T straight from the accumulators, rounded once to the products' type.
+// K rows lie 16 bytes and V rows 64 bytes further apart than they are long: both kinds of read then meet every bank once.
+// The maximum is only followed when it grows by more than 2^8: P is at most 256 then, its rounding is relative as before, and nearly all tiles skip
+// the rescaling of the sums.
+constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;
+constexpr float MANY_SLACK = 8.0f;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <bool F16> __device__ inline f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c)
+{
+    if (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ inline u32x2 lds_read_transposed(const char* p)
+{
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+    return __builtin_bit_cast(u32x2, x);
+}
+__device__ inline float halves_max(float x)
+{
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ inline float halves_sum(float x)
+{
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+template <int QT, int KVT, int DP> __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attention_many_kernel(AttnArgs a)
+{
+    constexpr bool F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
+    constexpr int K_PITCH = DP * 2 + 16, V_PITCH = DP * 2 + 64;
+    constexpr int ROW_LOADS = DP / (CODES ? 16 : 8);                            // 16-byte loads of a key row
+    constexpr int LOADS = MANY_KEYS * ROW_LOADS / (64 * MANY_WAVES);              // of a thread, for K and for V
+    __shared__ __align__(16) char s_k[2][MANY_KEYS * K_PITCH];
+    __shared__ __align__(16) char s_v[2][MANY_KEYS * V_PITCH];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x32 = lane & 31, half = lane >> 5;
+
+    // workgroups of one (sequence, K/V head) run on one XCD (consecutive workgroups go round the eight), next to each other: its keys stay in that L2
+    const int nbh = a.n * a.kv_heads, per_bh = a.tiles * a.nsplit;
+    int bh, id = (int)blockIdx.x;
+    if (nbh % 8 == 0) {
+        bh = id % 8 + id / 8 / per_bh * 8;
+        id = id / 8 % per_bh;
+    } else {
+        bh = id / per_bh;
+        id = id % per_bh;
+    }
+    const int split = id % a.nsplit, tile = a.tiles - 1 - id / a.nsplit;           // (causal: the longest rows first)
+    const int b = bh / a.kv_heads, h = bh % a.kv_heads;
+    const int len = keys_of(a, b), row0 = tile * MANY_ROWS;
+    int last_key = len;
+    if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + MANY_ROWS - 1, a.rows - 1) / a.group + 1));
+    const int all_tiles = (last_key + MANY_KEYS - 1) / MANY_KEYS, share = (all_tiles + a.nsplit - 1) / a.nsplit;
+    const int t0 = split * share, t1 = min(all_tiles, t0 + share);
+
+    // q as second operand (a negative factor is moved into it: exact)
+    const int r = row0 + 32 * wave + x32, rc = min(r, a.rows - 1);
+    const char* qp = a.q + (int64_t)b * a.q_stride[0] + (int64_t)(rc / a.group) * a.q_stride[1] + (int64_t)(h * a.group + rc % a.group) * a.q_stride[2];
+    const float c = fmaxf(fabsf(a.c), 1e-37f);                                        // (a factor of 0 must leave -infinity what it is)
+    u32x4 qf[DP / 16];
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) {
+        const int at = 16 * u + 8 * half;
+        qf[u] = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
+        if (a.c < 0) qf[u] ^= 0x80008000u;
+    }
+    const int lim = a.causal ? len - a.tq + rc / a.group + 1 : len;                 // this lane's row sees keys below it
+    int wave_lim = len, wave_first = len;                                             // the most and the fewest keys a row of this wave sees
+    if (a.causal) {
+        wave_first = len - a.tq + min(row0 + 32 * wave, a.rows - 1) / a.group + 1;
+        wave_lim = len - a.tq + min(row0 + 32 * wave + 31, a.rows - 1) / a.group + 1;
+    }
+
+    const char* kb = a.k + (int64_t)b * a.k_stride[0] + (int64_t)h * a.k_stride[2];
+    const char* vb = a.v + (int64_t)b * a.v_stride[0] + (int64_t)h * a.v_stride[2];
+    const float* ksc = CODES ? a.k_scale + (int64_t)bh * a.scale_stride : nullptr;
+    const float* vsc = CODES ? a.v_scale + (int64_t)bh * a.scale_stride : nullptr;
+    const uint8_t* pad = a.pad ? a.pad + (int64_t)b * a.pad_stride : nullptr;
+
+    u32x4 kr[LOADS], vr[LOADS];
+    uint64_t next_mask = 0;
+    float ks = 1.0f, vs = 1.0f;
+    // loads of tile t into registers; keys past the end are read from the last one
+    const auto fetch = [&](int t) {
+        const int c0 = t * MANY_KEYS;
+        next_mask = __ballot(c0 + lane < len && (!pad || pad[c0 + lane] == 0));
+        if constexpr (CODES) {
+            ks = ksc[t];
+            vs = vsc[t];
+        }
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int e = tid + u * 64 * MANY_WAVES, key = min(c0 + e / ROW_LOADS, len - 1), at = e % ROW_LOADS * 16;
+            const bool in = at < a.d * (CODES ? 1 : 2);
+            const uint64_t k64 = (uint64_t)(uint32_t)key;
+            kr[u] = in ? *reinterpret_cast<const u32x4*>(kb + k64 * (uint64_t)a.k_stride[1] + at) : u32x4{};
+            vr[u] = in ? *reinterpret_cast<const u32x4*>(vb + k64 * (uint64_t)a.v_stride[1] + at) : u32x4{};
+        }
+    };
+    // registers into LDS; what is not admitted may hold anything: V = 0 meets P = 0
+    const auto stage = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int e = tid + u * 64 * MANY_WAVES, row = e / ROW_LOADS, at = e % ROW_LOADS;
+            if (next_mask != ~0ull && !((next_mask >> row) & 1)) vr[u] = u32x4{};
+            if constexpr (CODES) {
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    u32x4 x, y;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        x[2 * j] = codes_bf16<false>(kr[u][2 * w + j], ks);
+                        x[2 * j + 1] = codes_bf16<true>(kr[u][2 * w + j], ks);
+                        y[2 * j] = codes_bf16<false>(vr[u][2 * w + j], vs);
+                        y[2 * j + 1] = codes_bf16<true>(vr[u][2 * w + j], vs);
+                    }
+                    *reinterpret_cast<u32x4*>(&s_k[buf][row * K_PITCH + at * 32 + 16 * w]) = x;
+                    *reinterpret_cast<u32x4*>(&s_v[buf][row * V_PITCH + at * 32 + 16 * w]) = y;
+                }
+            } else {
+                *reinterpret_cast<u32x4*>(&s_k[buf][row * K_PITCH + at * 16]) = kr[u];
+                *reinterpret_cast<u32x4*>(&s_v[buf][row * V_PITCH + at * 16]) = vr[u];
+            }
+        }
+    };
+
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
+    float m = NEG_INF, l = 0.0f;
+    uint64_t mask = 0;
+    if (t0 < t1) {
+        fetch(t0);
+        mask = next_mask;
+        stage(0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1, c0 = t * MANY_KEYS;
+        if (t + 1 < t1) fetch(t + 1);
+        if (mask != 0 && c0 < wave_lim) {
+            // S^T, 64 keys x 32 rows
+            f32x16 s[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                s[kt] = f32x16{};
+                const char* p = &s_k[buf][(32 * kt + x32) * K_PITCH + 16 * half];
+#pragma unroll
+                for (int u = 0; u < DP / 16; ++u) s[kt] = mfma32<F16>(*reinterpret_cast<const u32x4*>(p + 32 * u), qf[u], s[kt]);
+            }
+            if (mask != ~0ull || c0 + MANY_KEYS > wave_first) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
+                        s[kt][i] = ((mask >> key) & 1) && c0 + key < lim ? s[kt][i] : NEG_INF;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
+            top = halves_max(top) * c;
+            if (__ballot(top > m + MANY_SLACK || (m == NEG_INF && top > NEG_INF))) {
+                const float grown = fmaxf(m, top), f = rescale(m, grown);
+                m = grown;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i][j] *= f;
+            }
+            const float base = m == NEG_INF ? 0.0f : m;
+            float sum = 0.0f;
+            uint32_t pf[2][8];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i], c, -base)), p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i + 1], c, -base));
+                    sum += p0 + p1;
+                    pf[kt][i] = pack16<F16>(p0, p1);
+                }
+            l += sum;
+            // O^T: 16 keys at a time; lane group (lane / 16) reads four keys 4 half + 0 .. 3 and 8 later of columns 16 (group % 2) + 0 .. 15
+            const char* vp = &s_v[buf][(4 * half + ((lane & 15) >> 2)) * V_PITCH + 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3))];
+#pragma unroll
+            for (int k16 = 0; k16 < 4; ++k16) {
+                const u32x4 p = {pf[k16 >> 1][4 * (k16 & 1)], pf[k16 >> 1][4 * (k16 & 1) + 1], pf[k16 >> 1][4 * (k16 & 1) + 2], pf[k16 >> 1][4 * (k16 & 1) + 3]};
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) {
+                    const u32x2 lo = lds_read_transposed(vp + 16 * k16 * V_PITCH + 64 * i), hi = lds_read_transposed(vp + (16 * k16 + 8) * V_PITCH + 64 * i);
+                    o[i] = mfma32<F16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[i]);
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            mask = next_mask;
+            stage(buf ^ 1);
+        }
+        __syncthreads();
+    }
+
+    if (r >= a.rows) return;
+    const float sum = halves_sum(l);
+    if (a.nsplit > 1) {
+        float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
+        if (half == 0) { ws[0] = m; ws[1] = sum; }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = 32 * i + 8 * j + 4 * half;
+                if (at < a.d) *reinterpret_cast<f32x4*>(ws + 4 + at) = f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+            }
+        return;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] + (int64_t)(h * a.group + r % a.group) * a.out_stride[2];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = 32 * i + 8 * j + 4 * half;
+            if (at >= a.d) continue;
+            u32x2 w;
+            w[0] = pack16<QT == ASR_F16>(o[i][4 * j] * inv, o[i][4 * j + 1] * inv);
+            w[1] = pack16<QT == ASR_F16>(o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv);
+            *reinterpret_cast<u32x2*>(op + 2 * at) = w;
+        }
+}
+
 // joins the shares of a long key axis: one thread per four output values
 template <int QT> __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a)
 {
@@ -463,13 +705,26 @@ template <int QT> __global__ __launch_bounds__(256) void attention_join_kernel(A
 // ---- the choice of kernel -----------------------------------------------------------------------------------------------
 struct Plan {
     int rows, tiles, nq, nsplit;
+    bool many;
     int64_t ws_bytes;
 };
 
-Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d)
+// sixteen: 16-bit products of one term each (bf16 or f16 keys, or codes with a bf16 query)
+Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, bool sixteen)
 {
     Plan p{};
     p.rows = (int)(tq * (heads / kv_heads));
+    p.many = sixteen && p.rows > 32;
+    if (p.many) {
+        p.tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
+        const int64_t wgs = n * kv_heads * p.tiles, most = tk / (MANY_KEYS * 8);
+        int64_t split = wgs > 0 ? 512 / wgs : 1;
+        if (split > most) split = most;
+        if (split > 16) split = 16;
+        p.nsplit = split < 1 ? 1 : (int)split;
+        p.ws_bytes = p.nsplit > 1 ? (int64_t)p.nsplit * n * kv_heads * p.rows * (d + 4) * 4 : 0;
+        return p;
+    }
     p.nq = p.rows > 16 ? 2 : 1;
     p.tiles = (p.rows + 16 * p.nq - 1) / (16 * p.nq);
     // shares of the key axis: enough workgroups for the chip (two for each of 256 compute units), each with at least four chunks of 32 keys for each wave
@@ -489,6 +744,12 @@ template <int QT, int KVT> hipError_t launch_few(const AttnArgs& a, int nq, hipS
     return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 128, 1>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 128, 2>, grid, block, s, a);
 }
 
+template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, hipStream_t s)
+{
+    const dim3 grid((uint32_t)((int64_t)a.n * a.kv_heads * a.nsplit * a.tiles)), block(64 * MANY_WAVES);
+    return a.d <= 64 ? ops_launch(attention_many_kernel<QT, KVT, 64>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 128>, grid, block, s, a);
+}
+
 template <int QT> hipError_t launch_join(const AttnArgs& a, hipStream_t s)
 {
     const int64_t blocks = ((int64_t)a.n * a.kv_heads * a.rows * (a.d / 4) + 255) / 256;
@@ -505,7 +766,9 @@ template <int QT, int KVT> int attend(const char* what, AttnArgs& a, const Plan&
         if (reinterpret_cast<uintptr_t>(ws) & 15) return ops_fail(ASR_ERR_ARG, "%s: the workspace must be 16-byte aligned", what);
         a.ws = static_cast<float*>(ws);
     }
-    hipError_t e = launch_few<QT, KVT>(a, p.nq, s);
+    hipError_t e;
+    if constexpr (QT != ASR_F32 && !(QT == ASR_F16 && KVT == KV_E4M3)) e = p.many ? launch_many<QT, KVT>(a, s) : launch_few<QT, KVT>(a, p.nq, s);
+    else e = launch_few<QT, KVT>(a, p.nq, s);
     if (e == hipSuccess && p.nsplit > 1) e = launch_join<QT>(a, s);
     return ops_launched(what, e);
 }
@@ -532,7 +795,7 @@ extern "C" {
 int64_t asr_cross_attention_workspace(int32_t n, int32_t tq, int32_t tk, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype)
 {
     if (bad_sizes(n, tq, tk, heads, kv_heads, d, 8) || !ops_dtype_ok(dtype)) return 0;
-    return plan_of(n, tq, tk, heads, kv_heads, d).ws_bytes;
+    return plan_of(n, tq, tk, heads, kv_heads, d, dtype != ASR_F32).ws_bytes;
 }
 
 int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
@@ -540,7 +803,7 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
     if (!a) return ops_fail(ASR_ERR_ARG, "null argument");
     if (const char* why = bad_sizes(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d, 8)) return ops_fail(ASR_ERR_ARG, "cross_attention: %s", why);
     if (!ops_dtype_ok(a->dtype)) return ops_fail(ASR_ERR_ARG, "cross_attention: unknown dtype %d", a->dtype);
-    if (!isfinite(a->scale)) return ops_fail(ASR_ERR_ARG, "cross_attention: the scale must be finite");
+    if (!isfinite(a->scale * LOG2E)) return ops_fail(ASR_ERR_ARG, "cross_attention: the scale must be finite");
     if (a->n == 0 || a->tq == 0) return ASR_OK;
     if (!a->q || !a->out || (a->tk > 0 && (!a->k || !a->v))) return ops_fail(ASR_ERR_ARG, "cross_attention: null argument");
     if (!nonnegative(a->q_stride) || !nonnegative(a->k_stride) || !nonnegative(a->v_stride) || !nonnegative(a->out_stride) || a->pad_stride < 0)
@@ -560,7 +823,7 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
     }
     x.n = a->n; x.tq = a->tq; x.tk = a->tk; x.kv_heads = a->kv_heads; x.group = a->heads / a->kv_heads; x.d = a->d;
     x.c = a->scale * LOG2E;
-    const Plan p = plan_of(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d);
+    const Plan p = plan_of(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d, a->dtype != ASR_F32);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->dtype == ASR_F32) return attend<ASR_F32, KV_F32>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
     if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_BF16>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
@@ -570,7 +833,7 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
 int64_t asr_kv8_attention_workspace(int32_t n, int32_t tq, int32_t capacity, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype)
 {
     if (bad_sizes(n, tq, capacity, heads, kv_heads, d, 16) || !ops_dtype_ok(dtype)) return 0;
-    return plan_of(n, tq, capacity, heads, kv_heads, d).ws_bytes;
+    return plan_of(n, tq, capacity, heads, kv_heads, d, dtype == ASR_BF16).ws_bytes;
 }
 
 int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
@@ -579,7 +842,7 @@ int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
     if (const char* why = bad_sizes(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d, 16)) return ops_fail(ASR_ERR_ARG, "kv8_attention: %s", why);
     if (a->capacity % ASR_KV8_BLOCK) return ops_fail(ASR_ERR_ARG, "kv8_attention: the capacity must be a multiple of %d tokens", ASR_KV8_BLOCK);
     if (!ops_dtype_ok(a->dtype)) return ops_fail(ASR_ERR_ARG, "kv8_attention: unknown dtype %d", a->dtype);
-    if (!isfinite(a->scale)) return ops_fail(ASR_ERR_ARG, "kv8_attention: the scale must be finite");
+    if (!isfinite(a->scale * LOG2E)) return ops_fail(ASR_ERR_ARG, "kv8_attention: the scale must be finite");
     if (a->n == 0 || a->tq == 0) return ASR_OK;
     if (!a->q || !a->out || !a->lens || (a->capacity > 0 && (!a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale)))
         return ops_fail(ASR_ERR_ARG, "kv8_attention: null argument");
@@ -602,7 +865,7 @@ int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
     x.n = a->n; x.tq = a->tq; x.tk = a->capacity; x.kv_heads = a->kv_heads; x.group = a->heads / a->kv_heads; x.d = a->d;
     x.causal = a->causal ? 1 : 0;
     x.c = a->scale * LOG2E;
-    const Plan p = plan_of(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d);
+    const Plan p = plan_of(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d, a->dtype == ASR_BF16);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->dtype == ASR_F32) return attend<ASR_F32, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
     if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
