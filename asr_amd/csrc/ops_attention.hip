@@ -431,11 +431,13 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
 // buffers: the next tile's loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
 // scale).  32 x 32 x 16 products: S^T = K q^T has a row in each lane of 32 and lane half; O^T = V^T P^T takes V^T from LDS with the transposing read
 // (four keys of one column a lane) and P^T straight from the accumulators, rounded once to the products' type.
-// K rows lie 16 bytes and V rows 64 bytes further apart than they are long: both kinds of read then meet every bank once.
+// The 16-byte chunks of a row are permuted by its number (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4), by pairs of rows where rows are half
+// as long): both kinds of read then meet every bank evenly.  Rows of 16-bit values as long as the tile go from memory to LDS directly.
 // The maximum is only followed when it grows by more than 2^8: P is at most 256 then, its rounding is relative as before, and nearly all tiles skip
 // the rescaling of the sums.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;
 constexpr float MANY_SLACK = 8.0f;
+constexpr float MANY_NONE = -3.0e38f;        // maximum of a row that has seen no key: finite, so that no difference with it is NaN
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -450,6 +452,14 @@ __device__ inline u32x2 lds_read_transposed(const char* p)
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
     return __builtin_bit_cast(u32x2, x);
 }
+// 16 bytes a lane from memory to LDS, the wave's 1024 in lane order from `lds` on; done when the wave has waited for its memory operations.  (The
+// builtin would have every later LDS read wait for it, as the compiler cannot tell the buffers apart.)
+__device__ inline void load_to_lds(const char* p, char* lds)
+{
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory");
+}
+__device__ inline void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ inline float halves_max(float x)
 {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -461,15 +471,26 @@ __device__ inline float halves_sum(float x)
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-template <int QT, int KVT, int DP> __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attention_many_kernel(AttnArgs a)
+// dot product of two 16-bit pairs with (1, 1), added to c: the sum of two probabilities as they are multiplied
+template <bool F16> __device__ inline float pair_sum(uint32_t w, float c)
+{
+    if (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+}
+
+template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attention_many_kernel(AttnArgs a)
 {
     constexpr bool F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
-    constexpr int K_PITCH = DP * 2 + 16, V_PITCH = DP * 2 + 64;
+    constexpr bool DIRECT = FULL && !CODES;
+    constexpr int PITCH = DP * 2, PAIR = 128 / DP;
     constexpr int ROW_LOADS = DP / (CODES ? 16 : 8);                            // 16-byte loads of a key row
     constexpr int LOADS = MANY_KEYS * ROW_LOADS / (64 * MANY_WAVES);              // of a thread, for K and for V
-    __shared__ __align__(16) char s_k[2][MANY_KEYS * K_PITCH];
-    __shared__ __align__(16) char s_v[2][MANY_KEYS * V_PITCH];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x32 = lane & 31, half = lane >> 5;
+    constexpr int LOAD_ROWS = 64 * MANY_WAVES / ROW_LOADS;                        // rows from one load of a thread to its next (a multiple of 16)
+    __shared__ __align__(16) char s_k[3][MANY_KEYS * PITCH];
+    __shared__ __align__(16) char s_v[2][MANY_KEYS * PITCH];
+    const auto turn_k = [](int row) { return (row / PAIR) & (DP / 8 - 1); };                 // of a row's 16-byte chunks
+    const auto turn_v = [](int row) { return PAIR == 1 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); };
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x32 = lane & 31, half = lane >> 5;
 
     // workgroups of one (sequence, K/V head) run on one XCD (consecutive workgroups go round the eight), next to each other: its keys stay in that L2
     const int nbh = a.n * a.kv_heads, per_bh = a.tiles * a.nsplit;
@@ -513,130 +534,258 @@ template <int QT, int KVT, int DP> __global__ __launch_bounds__(64 * MANY_WAVES,
     const float* vsc = CODES ? a.v_scale + (int64_t)bh * a.scale_stride : nullptr;
     const uint8_t* pad = a.pad ? a.pad + (int64_t)b * a.pad_stride : nullptr;
 
-    u32x4 kr[LOADS], vr[LOADS];
-    uint64_t next_mask = 0;
+    // this thread's place in a tile: row and 16-byte load of it
+    const int my_row = tid / ROW_LOADS, my_load = tid % ROW_LOADS;
+    const int k_at = DIRECT ? (my_load ^ turn_k(my_row)) * 16 : my_load * 16, v_at = DIRECT ? (my_load ^ turn_v(my_row)) * 16 : my_load * 16;
+    const bool in = FULL || my_load * 16 < a.d * (CODES ? 1 : 2);
+    const char* kp = kb + (uint64_t)my_row * (uint64_t)a.k_stride[1] + (in ? k_at : 0);
+    const char* vp = vb + (uint64_t)my_row * (uint64_t)a.v_stride[1] + (in ? v_at : 0);
+
+    const int64_t k_step = LOAD_ROWS * a.k_stride[1], v_step = LOAD_ROWS * a.v_stride[1];
+
+    u32x4 kr[DIRECT ? 1 : LOADS], vr[DIRECT ? 1 : LOADS];
     float ks = 1.0f, vs = 1.0f;
-    // loads of tile t into registers; keys past the end are read from the last one
-    const auto fetch = [&](int t) {
+    // one bit for each admitted key of tile t
+    const auto admitted = [&](int t) __attribute__((always_inline)) {
+        if (!pad && (t + 1) * MANY_KEYS <= len) return ~(uint64_t)0;
+        const int key = t * MANY_KEYS + lane;
+        return (uint64_t)__ballot(key < len && (!pad || pad[key] == 0));
+    };
+    // where this thread's loads of tile t of K or V come from (p: its first row's place in that tile); keys past the end are read from the last one
+    const auto aim = [&](int t, const char* p, int64_t stride, int64_t step, const char* (&x)[LOADS]) __attribute__((always_inline)) {
         const int c0 = t * MANY_KEYS;
-        next_mask = __ballot(c0 + lane < len && (!pad || pad[c0 + lane] == 0));
-        if constexpr (CODES) {
-            ks = ksc[t];
-            vs = vsc[t];
-        }
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int e = tid + u * 64 * MANY_WAVES, key = min(c0 + e / ROW_LOADS, len - 1), at = e % ROW_LOADS * 16;
-            const bool in = at < a.d * (CODES ? 1 : 2);
-            const uint64_t k64 = (uint64_t)(uint32_t)key;
-            kr[u] = in ? *reinterpret_cast<const u32x4*>(kb + k64 * (uint64_t)a.k_stride[1] + at) : u32x4{};
-            vr[u] = in ? *reinterpret_cast<const u32x4*>(vb + k64 * (uint64_t)a.v_stride[1] + at) : u32x4{};
+        for (int u = 0; u < LOADS; ++u) x[u] = u ? x[u - 1] + step : p;
+        if (c0 + MANY_KEYS > len) {
+            asm volatile("");                                                       // (a branch: products of 64 bits in the last tile only)
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) x[u] += (int64_t)min(0, len - 1 - (c0 + u * LOAD_ROWS + my_row)) * stride;
         }
     };
-    // registers into LDS; what is not admitted may hold anything: V = 0 meets P = 0
-    const auto stage = [&](int buf) {
+    // ... load u of them, to registers or LDS
+    const auto load = [&](const char* const (&x)[LOADS], int u, u32x4* regs, char* lds) __attribute__((always_inline)) {
+        if constexpr (DIRECT) load_to_lds(x[u], lds + (u * MANY_WAVES + wave) * 1024);
+        else regs[u] = *reinterpret_cast<const u32x4*>(x[u]);
+    };
+    // fetched registers into LDS (the caller waits and meets the other waves afterwards)
+    const auto put = [&](u32x4* regs, char* lds, float scale, auto turn) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-            const int e = tid + u * 64 * MANY_WAVES, row = e / ROW_LOADS, at = e % ROW_LOADS;
-            if (next_mask != ~0ull && !((next_mask >> row) & 1)) vr[u] = u32x4{};
+            char* row = lds + (my_row + u * LOAD_ROWS) * PITCH;
+            if (!in) regs[u] = u32x4{};
             if constexpr (CODES) {
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    u32x4 x, y;
+                    u32x4 x;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        x[2 * j] = codes_bf16<false>(kr[u][2 * w + j], ks);
-                        x[2 * j + 1] = codes_bf16<true>(kr[u][2 * w + j], ks);
-                        y[2 * j] = codes_bf16<false>(vr[u][2 * w + j], vs);
-                        y[2 * j + 1] = codes_bf16<true>(vr[u][2 * w + j], vs);
+                        x[2 * j] = codes_bf16<false>(regs[u][2 * w + j], scale);
+                        x[2 * j + 1] = codes_bf16<true>(regs[u][2 * w + j], scale);
                     }
-                    *reinterpret_cast<u32x4*>(&s_k[buf][row * K_PITCH + at * 32 + 16 * w]) = x;
-                    *reinterpret_cast<u32x4*>(&s_v[buf][row * V_PITCH + at * 32 + 16 * w]) = y;
+                    *reinterpret_cast<u32x4*>(row + ((2 * my_load + w) ^ turn(my_row)) * 16) = x;
                 }
-            } else {
-                *reinterpret_cast<u32x4*>(&s_k[buf][row * K_PITCH + at * 16]) = kr[u];
-                *reinterpret_cast<u32x4*>(&s_v[buf][row * V_PITCH + at * 16]) = vr[u];
-            }
+            } else *reinterpret_cast<u32x4*>(row + (my_load ^ turn(my_row)) * 16) = regs[u];
         }
     };
+    const auto put_k = [&](int buf) __attribute__((always_inline)) {
+        if constexpr (!DIRECT) put(kr, s_k[buf], ks, turn_k);
+    };
+    // what is not admitted may hold anything: V = 0 meets P = 0
+    const auto put_v = [&](int t, uint64_t mask) __attribute__((always_inline)) {
+        if constexpr (DIRECT) {
+            if (mask == ~0ull) return;
+            wait_for_memory();                                                      // (a thread clears what its own loads brought)
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u)
+                if (!((mask >> (my_row + u * LOAD_ROWS)) & 1)) *reinterpret_cast<u32x4*>(&s_v[t & 1][(tid + u * 64 * MANY_WAVES) * 16]) = u32x4{};
+        } else {
+            if (mask != ~0ull) {
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u)
+                    if (!((mask >> (my_row + u * LOAD_ROWS)) & 1)) vr[u] = u32x4{};
+            }
+            put(vr, s_v[t & 1], vs, turn_v);
+        }
+    };
+    const auto meet = [&]() __attribute__((always_inline)) {
+        wait_for_memory();
+        __syncthreads();
+    };
 
+    // where the reads of a tile go: K row x32 of a half, 16-byte chunk 2 u + half of it; V: lane group lane / 16 reads four keys, 4 half + 0 .. 3, of columns
+    // 16 (group % 2) + 0 .. 15, its lane i key i / 4 and four columns from 4 (i % 4)
+    const int k_read = x32 * PITCH + 16 * (half ^ turn_k(x32)), v_row = 4 * half + ((lane & 15) >> 2);
+    const int v_read = v_row * PITCH + 8 * (lane & 1) + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ turn_v(v_row));
     f32x16 o[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
-    float m = NEG_INF, l = 0.0f;
+    float m = MANY_NONE, l = 0.0f;
     uint64_t mask = 0;
+    constexpr int AHEAD = 4, N = DP / 16, PAIRS = 8 / N;                             // N products of a half's scores, and of its output
+    u32x4 kf[N];                                                                     // of the next half's scores, AHEAD of them read beforehand
+
+    const auto scores = [&](const char* k_tile, int sub, f32x16& s) __attribute__((always_inline)) {
+        s = f32x16{};
+#pragma unroll
+        for (int u = 0; u < DP / 16; ++u) s = mfma32<F16>(*reinterpret_cast<const u32x4*>(k_tile + 32 * sub * PITCH + (k_read ^ (32 * u))), qf[u], s);
+    };
+    const auto k_frag = [&](const char* k_half, int u) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4*>(k_half + (k_read ^ (32 * u))); };
+    const auto most = [&](const f32x16& s) __attribute__((always_inline)) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        return halves_max(top) * c;
+    };
+    // soft-max and output of half `sub` of tile t from its scores s with their maximum `top`, and the scores of the half behind it: the matrix pipe
+    // computes those while the exponentials run, and the output while their maximum is taken.  The next tiles' loads go out one at a time in between
+    // (all at once they fill the memory pipe's queue and the wave waits: 1060 of 3500 cycles a tile).
+    const auto step = [&](int t, int sub, f32x16& s, float& top, const char* next_tile, const char* k_half_after, f32x16& next, const char* const (&from)[LOADS], u32x4* regs,
+                          char* to) __attribute__((always_inline)) {
+        const int c0 = t * MANY_KEYS + 32 * sub;
+        const uint32_t bits = (uint32_t)(mask >> (32 * sub));
+        if (bits != ~0u || c0 + 32 > wave_first) {
+            asm volatile("");                                                       // (a branch, not 16 selects in every step)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 8 * (i >> 2) + 4 * half + (i & 3);
+                s[i] = ((bits >> key) & 1) && c0 + key < lim ? s[i] : NEG_INF;
+            }
+            top = most(s);
+        }
+        if (__ballot(top > m + MANY_SLACK)) {
+            const float grown = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - grown);
+            m = grown;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[i][j] *= f;
+        }
+        // In the order in which it is to be issued (the compiler left to itself puts all products on one side): an LDS read AHEAD products before its own
+        // product, between the products their share of the exponentials - each value a stage further a product later, so that none waits for the
+        // one before - then of the maximum
+        const char *k_half = next_tile + 32 * (sub ^ 1) * PITCH, *v_half = s_v[t & 1] + 32 * sub * PITCH;
+        const auto v_frag = [&](int q) __attribute__((always_inline)) {
+            const char* p = v_half + 16 * (q / (N / 2)) * PITCH + (v_read ^ (64 * (q % (N / 2))));
+            const u32x2 lo = lds_read_transposed(p), hi = lds_read_transposed(p + 8 * PITCH);
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
+        u32x4 vf[N];
+        float x[16];
+        uint32_t pf[8];
+        float sum = 0.0f;
+        next = f32x16{};
+#pragma unroll
+        for (int j = 0; j < 2 * PAIRS; ++j) x[j] = fmaf(s[j], c, -m);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            if (u + AHEAD < N) kf[u + AHEAD] = k_frag(k_half, u + AHEAD);
+            else vf[u + AHEAD - N] = v_frag(u + AHEAD - N);
+            next = mfma32<F16>(kf[u], qf[u], next);
+            if (u % (N / LOADS) == 0 && u / (N / LOADS) < LOADS) load(from, u / (N / LOADS), regs, to);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 2 * PAIRS * u; j < 2 * PAIRS * (u + 1); ++j) {
+                if (j + 2 * PAIRS < 16) x[j + 2 * PAIRS] = fmaf(s[j + 2 * PAIRS], c, -m);
+                x[j] = __builtin_amdgcn_exp2f(x[j]);
+            }
+            if (u > 0) {
+#pragma unroll
+                for (int i = PAIRS * (u - 1); i < PAIRS * u; ++i) {
+                    pf[i] = pack16<F16>(x[2 * i], x[2 * i + 1]);
+                    sum = pair_sum<F16>(pf[i], sum);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float most_of[2];
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const int k16 = q / (N / 2), i = q % (N / 2);
+            if (q + AHEAD < N) vf[q + AHEAD] = v_frag(q + AHEAD);
+            else kf[q + AHEAD - N] = k_frag(k_half_after, q + AHEAD - N);
+            if (q == 0) {
+#pragma unroll
+                for (int j = PAIRS * (N - 1); j < 8; ++j) {
+                    pf[j] = pack16<F16>(x[2 * j], x[2 * j + 1]);
+                    sum = pair_sum<F16>(pf[j], sum);
+                }
+            }
+            o[i] = mfma32<F16>(vf[q], u32x4{pf[4 * k16], pf[4 * k16 + 1], pf[4 * k16 + 2], pf[4 * k16 + 3]}, o[i]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (q == N / 2) {
+                most_of[0] = next[0];
+                most_of[1] = next[1];
+            }
+            if (q >= N / 2) {
+#pragma unroll
+                for (int j = 32 * (q - N / 2) / N; j < 32 * (q + 1 - N / 2) / N; j += 4) {
+                    most_of[0] = fmaxf(fmaxf(most_of[0], next[j]), next[j + 2]);
+                    most_of[1] = fmaxf(fmaxf(most_of[1], next[j + 1]), next[j + 3]);
+                }
+                asm volatile("" : "+v"(most_of[0]), "+v"(most_of[1]));                  // (here, not behind the last product)
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum;
+        top = halves_max(fmaxf(most_of[0], most_of[1])) * c;
+    };
+
     if (t0 < t1) {
-        fetch(t0);
-        mask = next_mask;
-        stage(0);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1, c0 = t * MANY_KEYS;
-        if (t + 1 < t1) fetch(t + 1);
-        if (mask != 0 && c0 < wave_lim) {
-            // S^T, 64 keys x 32 rows
-            f32x16 s[2];
+        f32x16 sa, sb;
+        const char* from[LOADS];
+        int now = 0, behind = 1, fetched = 2;                                           // K buffers of tiles t, t + 1, t + 2
+        mask = admitted(t0);
+        // this thread's first row of the tile that is loaded next
+        const char *k_from = kp + (int64_t)t0 * MANY_KEYS * a.k_stride[1], *v_from = vp + (int64_t)t0 * MANY_KEYS * a.v_stride[1];
+        const int64_t k_tile = MANY_KEYS * a.k_stride[1], v_tile = MANY_KEYS * a.v_stride[1];
+        const auto bring_k = [&](int t, int buf) __attribute__((always_inline)) {
+            aim(t, k_from, a.k_stride[1], k_step, from);
+            if constexpr (CODES) ks = ksc[t];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                s[kt] = f32x16{};
-                const char* p = &s_k[buf][(32 * kt + x32) * K_PITCH + 16 * half];
+            for (int u = 0; u < LOADS; ++u) load(from, u, kr, s_k[buf]);
+            put_k(buf);
+        };
+        bring_k(t0, now);
+        aim(t0, v_from, a.v_stride[1], v_step, from);
+        if constexpr (CODES) vs = vsc[t0];
 #pragma unroll
-                for (int u = 0; u < DP / 16; ++u) s[kt] = mfma32<F16>(*reinterpret_cast<const u32x4*>(p + 32 * u), qf[u], s[kt]);
-            }
-            if (mask != ~0ull || c0 + MANY_KEYS > wave_first) {
+        for (int u = 0; u < LOADS; ++u) load(from, u, vr, s_v[t0 & 1]);
+        put_v(t0, mask);
+        if (t0 + 1 < t1) {
+            k_from += k_tile;
+            bring_k(t0 + 1, behind);
+        }
+        meet();
+        scores(s_k[now], 0, sa);
+        float top = most(sa);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
-                        s[kt][i] = ((mask >> key) & 1) && c0 + key < lim ? s[kt][i] : NEG_INF;
-                    }
-            }
-            float top = s[0][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
-            top = halves_max(top) * c;
-            if (__ballot(top > m + MANY_SLACK || (m == NEG_INF && top > NEG_INF))) {
-                const float grown = fmaxf(m, top), f = rescale(m, grown);
-                m = grown;
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i][j] *= f;
-            }
-            const float base = m == NEG_INF ? 0.0f : m;
-            float sum = 0.0f;
-            uint32_t pf[2][8];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i], c, -base)), p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i + 1], c, -base));
-                    sum += p0 + p1;
-                    pf[kt][i] = pack16<F16>(p0, p1);
-                }
-            l += sum;
-            // O^T: 16 keys at a time; lane group (lane / 16) reads four keys 4 half + 0 .. 3 and 8 later of columns 16 (group % 2) + 0 .. 15
-            const char* vp = &s_v[buf][(4 * half + ((lane & 15) >> 2)) * V_PITCH + 2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3))];
-#pragma unroll
-            for (int k16 = 0; k16 < 4; ++k16) {
-                const u32x4 p = {pf[k16 >> 1][4 * (k16 & 1)], pf[k16 >> 1][4 * (k16 & 1) + 1], pf[k16 >> 1][4 * (k16 & 1) + 2], pf[k16 >> 1][4 * (k16 & 1) + 3]};
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
-                    const u32x2 lo = lds_read_transposed(vp + 16 * k16 * V_PITCH + 64 * i), hi = lds_read_transposed(vp + (16 * k16 + 8) * V_PITCH + 64 * i);
-                    o[i] = mfma32<F16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[i]);
-                }
+        for (int u = 0; u < AHEAD; ++u) kf[u] = k_frag(s_k[now] + 32 * PITCH, u);
+        for (int t = t0; t < t1; ++t) {
+            // (behind the last tile the last one is loaded again, and scores are taken of what LDS holds: neither is used)
+            const int tk = min(t + 2, t1 - 1), tv = min(t + 1, t1 - 1);
+            const uint64_t next_mask = admitted(tv);
+            if (t + 2 < t1) k_from += k_tile;
+            if (t + 1 < t1) v_from += v_tile;
+            aim(tk, k_from, a.k_stride[1], k_step, from);
+            if constexpr (CODES) ks = ksc[tk];
+            step(t, 0, sa, top, s_k[now], s_k[behind], sb, from, kr, s_k[fetched]);
+            aim(tv, v_from, a.v_stride[1], v_step, from);
+            if constexpr (CODES) vs = vsc[tv];
+            step(t, 1, sb, top, s_k[behind], s_k[behind] + 32 * PITCH, sa, from, vr, s_v[(t + 1) & 1]);
+            if (t + 1 < t1) {
+                put_k(fetched);
+                put_v(t + 1, next_mask);
+                mask = next_mask;
+                meet();
+                const int free = now;
+                now = behind;
+                behind = fetched;
+                fetched = free;
             }
         }
-        if (t + 1 < t1) {
-            mask = next_mask;
-            stage(buf ^ 1);
-        }
-        __syncthreads();
+        wait_for_memory();                                                              // (no load into LDS may outlive its workgroup)
     }
 
     if (r >= a.rows) return;
@@ -747,7 +896,9 @@ template <int QT, int KVT> hipError_t launch_few(const AttnArgs& a, int nq, hipS
 template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, hipStream_t s)
 {
     const dim3 grid((uint32_t)((int64_t)a.n * a.kv_heads * a.nsplit * a.tiles)), block(64 * MANY_WAVES);
-    return a.d <= 64 ? ops_launch(attention_many_kernel<QT, KVT, 64>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 128>, grid, block, s, a);
+    if (a.d == 64) return ops_launch(attention_many_kernel<QT, KVT, 64, true>, grid, block, s, a);
+    if (a.d == 128) return ops_launch(attention_many_kernel<QT, KVT, 128, true>, grid, block, s, a);
+    return a.d < 64 ? ops_launch(attention_many_kernel<QT, KVT, 64, false>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 128, false>, grid, block, s, a);
 }
 
 template <int QT> hipError_t launch_join(const AttnArgs& a, hipStream_t s)
