@@ -41,6 +41,10 @@ struct AttnArgs {
     float c;                             // scale * log2(e): powers of two instead of e
 };
 
+// a place in GPU memory: where pointers are chosen between, the compiler no longer sees that they are none of LDS and takes slower loads
+typedef const __attribute__((address_space(1))) char* mem;
+template <typename T> __device__ inline T load_as(mem p) { return *(const __attribute__((address_space(1))) T*)p; }
+
 __device__ inline uint32_t pack_bf16(float a, float b)
 {
     bf16x2 r;
@@ -96,8 +100,10 @@ __device__ inline float groups_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// e^(m_old - m_new) as a power of two of the scaled scores; 0 where nothing was summed yet
-__device__ inline float rescale(float m_old, float m_new) { return m_old == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_old - m_new); }
+// m follows a row's maximum (in powers of two) only when that grows by more than SLACK: P is at most 2^SLACK then, its rounding is relative as before, and
+// nearly all tiles skip the scaling of the sums.  It starts finite, so that no difference with it is NaN.
+constexpr float SLACK = 8.0f, NO_MAX = -3.0e38f;
+__device__ inline float rescale(float m_old, float m_new) { return __builtin_amdgcn_exp2f(m_old - m_new); }
 
 __device__ inline int keys_of(const AttnArgs& a, int b) { return a.lens ? min(max(a.lens[b], 0), a.tk) : a.tk; }
 
@@ -121,8 +127,9 @@ __device__ inline int place_of(int nbh, int per, int64_t& id)
 
 // ---- few rows: the waves of a workgroup share the keys ------------------------------------------------------------------
 // A workgroup has one tile of 16 NQ rows of one (sequence, K/V head) and one share of its keys; its four waves take 32 keys at a time in turn,
-// straight from memory into registers in the operands' own order (no LDS in the loop), and join their sums in LDS at the end.  K and V are
-// read once by each row tile: bound by those bytes while there are few rows.  QT: type of q and out, KVT: of K and V.
+// straight from memory into registers in the operands' own order (no LDS in the loop), and join their sums in LDS at the end.  The next chunk's
+// keys are loaded as soon as the scores have been taken from this one's, the next values behind the output.  K and V are read once by each row
+// tile: bound by those bytes while there are few rows.  QT: type of q and out, KVT: of K and V.
 // Terms: 16-bit K / V are exact factors; q enters as QTERMS 16-bit terms (bf16 codes: f16 = 2, f32 = 3 bf16 terms lose nothing) and
 // P as PTERMS (two: 2^-17 / 2^-22 of it lost, three: nothing), which costs matrix instructions that a loop waiting for memory has to spare.
 template <int QT, int KVT, int DP, int NQ> struct Few {
@@ -133,6 +140,7 @@ template <int QT, int KVT, int DP, int NQ> struct Few {
     static constexpr int QB = QT == ASR_F32 ? 4 : 2;
     static constexpr int KW = DP / 4 * KVB / 4;                             // words of a key row in one lane (a quarter of it)
     static constexpr int VW = DP / 16 * KVB / 4;                            // words of a value row in one lane (a sixteenth)
+    typedef uint32_t VRow __attribute__((ext_vector_type(VW)));
     static constexpr int NO = DP / 16;                                      // 16 x 16 output tiles of one row tile
 };
 
@@ -144,13 +152,13 @@ template <int KVT> __device__ constexpr int quarter_at(int g, int j)
     return KVT == KV_F32 ? 16 * (j >> 2) + 4 * g + (j & 3) : KVT == KV_E4M3 ? 64 * (j >> 4) + 16 * g + (j & 15) : 32 * (j >> 3) + 8 * g + (j & 7);
 }
 
-template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW_WAVES) void attention_few_kernel(AttnArgs a)
+template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds__(64 * FEW_WAVES) void attention_few_kernel(AttnArgs a)
 {
     typedef Few<QT, KVT, DP, NQ> F;
     constexpr int PITCH = DP + 4;
     __shared__ float s_m[FEW_WAVES][16 * NQ], s_l[FEW_WAVES][16 * NQ];
     __shared__ __align__(16) float s_o[FEW_WAVES][16 * NQ][PITCH];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x16 = lane & 15, g = lane >> 4;
     int64_t id = blockIdx.x;
     const int bh = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
     const int split = (int)(id % a.nsplit), tile = (int)(id / a.nsplit);
@@ -215,7 +223,7 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
     float m[NQ], l[NQ];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-        m[t] = NEG_INF;
+        m[t] = NO_MAX;
         l[t] = 0.0f;
 #pragma unroll
         for (int i = 0; i < F::NO; ++i) o[t][i] = f32x4{};
@@ -227,70 +235,72 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
         ksc = a.k_scale + (int64_t)bh * a.scale_stride;
         vsc = a.v_scale + (int64_t)bh * a.scale_stride;
     }
-    const bool full = a.d == DP;
+    const uint8_t* pad = a.pad ? a.pad + (int64_t)b * a.pad_stride : nullptr;
 
-    for (int chunk = chunk0 + wave; chunk < chunk1; chunk += FEW_WAVES) {
-        const int c0 = chunk * 32;
-        // one admitted-bit per key of the chunk, the same for the whole wave
-        const int mk = c0 + (lane & 31);
-        const bool ok = mk < len && (!a.pad || a.pad[(int64_t)b * a.pad_stride + mk] == 0);
-        const uint32_t mask = (uint32_t)__ballot(ok);
-        if (mask == 0) continue;
-        const uint32_t mine = mask >> (8 * g);                                 // bits 0 .. 7: keys 8 g .. 8 g + 7
-
-        // K: tile t2's row x16 is key 8 (x16 / 4) + 4 t2 + x16 % 4; V: lane group g has keys 8 g .. 8 g + 7, lane x16 a sixteenth of each row.
-        // Keys past the end are read from the last one.
-        uint32_t kr[2][F::KW], vr[8][F::VW];
+    // K: tile t2's row x16 is key 8 (x16 / 4) + 4 t2 + x16 % 4 of a chunk; V: lane group g has keys 8 g .. 8 g + 7, lane x16 a sixteenth of each row.
+    // Keys past the end are read from the last one; values past d are zeros (K) or not used (V).
+    const int k_row = 8 * (x16 >> 2) + (x16 & 3), v_row = 8 * g;
+    const int v_at = F::MATH32 ? 4 * x16 : DP / 16 * x16;
+    const mem kp = (mem)(kb + (uint64_t)k_row * (uint64_t)a.k_stride[1]);
+    const mem vp = (mem)(vb + (uint64_t)v_row * (uint64_t)a.v_stride[1] + (FULL || v_at < a.d ? v_at * F::KVB : 0));
+    u32x4 kr[2][F::KW / 4];                        // (vectors as they are loaded: taken apart into words here, pairs of them were given one register)
+    typename F::VRow vr[8];
+    uint32_t flag = 0;
+    float ks = 1.0f, vs = 1.0f;
+    const auto load_k = [&](int c0) __attribute__((always_inline)) {
+        if (pad) flag = c0 + (lane & 31) < len ? pad[c0 + (lane & 31)] : 0;
+        if constexpr (F::CODES) ks = ksc[c0 / ASR_KV8_BLOCK];
+        mem p[2];
 #pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {
-            const int key = min(c0 + 8 * (x16 >> 2) + 4 * t2 + (x16 & 3), len - 1);
-            const char* p = kb + (uint64_t)(uint32_t)key * (uint64_t)a.k_stride[1];
+        for (int t2 = 0; t2 < 2; ++t2) p[t2] = kp + (c0 + 4 * t2) * a.k_stride[1];
+        if (c0 + 32 > len) {
+            asm volatile("");                                                  // (a branch: products of 64 bits in the last chunk only)
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2) p[t2] += (int64_t)min(0, len - 1 - (c0 + 4 * t2 + k_row)) * a.k_stride[1];
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
             for (int w = 0; w < F::KW; w += 4) {
                 const int at = quarter_at<KVT>(g, w * 4 / F::KVB);
-                const u32x4 x = *reinterpret_cast<const u32x4*>(p + (full || at < a.d ? at * F::KVB : 0));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) kr[t2][w + j] = full || at < a.d ? x[j] : 0u;
+                kr[t2][w / 4] = load_as<u32x4>(p[t2] + (FULL || at < a.d ? at * F::KVB : 0));
+                if (!FULL && at >= a.d) kr[t2][w / 4] = u32x4{};
             }
+    };
+    const auto load_v = [&](int c0) __attribute__((always_inline)) {
+        if constexpr (F::CODES) vs = vsc[c0 / ASR_KV8_BLOCK];
+        mem p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = vp + (c0 + j) * a.v_stride[1];
+        if (c0 + 32 > len) {
+            asm volatile("");
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] += (int64_t)min(0, len - 1 - (c0 + j + v_row)) * a.v_stride[1];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int key = min(c0 + 8 * g + j, len - 1);
-            const char* p = vb + (uint64_t)(uint32_t)key * (uint64_t)a.v_stride[1];
             if constexpr (F::MATH32) {
 #pragma unroll
                 for (int u = 0; u < DP / 64; ++u) {
-                    const int at = 64 * u + 4 * x16;
-                    const u32x4 x = *reinterpret_cast<const u32x4*>(p + (full || at < a.d ? at * 4 : 0));
+                    const u32x4 x = load_as<u32x4>(p[j] + (FULL || 64 * u + v_at < a.d ? 256 * u : 0));
 #pragma unroll
                     for (int w = 0; w < 4; ++w) vr[j][4 * u + w] = x[w];
                 }
-            } else {
-                const int at = DP / 16 * x16;
-                p += full || at < a.d ? at * F::KVB : 0;
-                if constexpr (F::VW == 4) {
-                    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) vr[j][w] = x[w];
-                } else if constexpr (F::VW == 2) {
-                    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-                    vr[j][0] = x[0];
-                    vr[j][1] = x[1];
-                } else vr[j][0] = *reinterpret_cast<const uint32_t*>(p);
-            }
+            } else vr[j] = load_as<typename F::VRow>(p[j]);
         }
-        if (mask != 0xffffffffu) {                                             // what is not admitted may hold anything: P = 0 meets V = 0
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int w = 0; w < F::VW; ++w) vr[j][w] = (mine >> j) & 1 ? vr[j][w] : 0u;
-        }
-        float ks = 1.0f, vs = 1.0f;
-        if constexpr (F::CODES) {
-            ks = ksc[c0 / ASR_KV8_BLOCK];
-            vs = vsc[c0 / ASR_KV8_BLOCK];
-        }
+    };
 
+    int chunk = chunk0 + wave;
+    if (chunk < chunk1) {
+        load_k(32 * chunk);
+        load_v(32 * chunk);
+    }
+    for (; chunk < chunk1; chunk += FEW_WAVES) {
+        const int c0 = chunk * 32;
+        const bool more = chunk + FEW_WAVES < chunk1;
+        // one admitted-bit per key of the chunk, the same for the whole wave
+        const uint32_t mask = (uint32_t)__ballot(c0 + (lane & 31) < len && flag == 0);
+        const uint32_t mine = mask >> (8 * g);                                 // bits 0 .. 7: keys 8 g .. 8 g + 7
         // S^T
         f32x4 s[NQ][2];
 #pragma unroll
@@ -302,20 +312,15 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
                 for (int w = 0; w < F::KW; ++w)
 #pragma unroll
                     for (int t = 0; t < NQ; ++t)
-                        s[t][t2] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t2][w]), __uint_as_float(qf[t][0][w / 4][w % 4]), s[t][t2], 0, 0, 0);
+                        s[t][t2] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t2][w / 4][w % 4]), __uint_as_float(qf[t][0][w / 4][w % 4]), s[t][t2], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int u = 0; u < DP / 32; ++u) {
                     u32x4 kf;
                     if constexpr (F::CODES) {
-                        kf[0] = codes_bf16<false>(kr[t2][2 * u], ks);
-                        kf[1] = codes_bf16<true>(kr[t2][2 * u], ks);
-                        kf[2] = codes_bf16<false>(kr[t2][2 * u + 1], ks);
-                        kf[3] = codes_bf16<true>(kr[t2][2 * u + 1], ks);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) kf[j] = kr[t2][4 * u + j];
-                    }
+                        const uint32_t lo = kr[t2][u / 2][2 * (u & 1)], hi = kr[t2][u / 2][2 * (u & 1) + 1];
+                        kf = u32x4{codes_bf16<false>(lo, ks), codes_bf16<true>(lo, ks), codes_bf16<false>(hi, ks), codes_bf16<true>(hi, ks)};
+                    } else kf = kr[t2][u];
 #pragma unroll
                     for (int term = F::QTERMS - 1; term >= 0; --term)
 #pragma unroll
@@ -324,6 +329,8 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
             }
         }
 
+        if (more) load_k(c0 + 32 * FEW_WAVES);
+
         // soft-max step; p[t][4 t2 + i] belongs to key 8 g + 4 t2 + i
         float p[NQ][8];
 #pragma unroll
@@ -331,27 +338,35 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[t][j] = s[t][j >> 2][j & 3] * a.c;
             if (mask != 0xffffffffu || a.causal) {
+                asm volatile("");
 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[t][j] = ((mine >> j) & 1) && c0 + 8 * g + j < lim[t] ? p[t][j] : NEG_INF;
             }
             float top = p[t][0];
 #pragma unroll
             for (int j = 1; j < 8; ++j) top = fmaxf(top, p[t][j]);
-            top = fmaxf(m[t], groups_max(top));
-            const float f = rescale(m[t], top), base = top == NEG_INF ? 0.0f : top;
-            m[t] = top;
+            top = groups_max(top);
+            if (__ballot(top > m[t] + SLACK)) {
+                const float grown = fmaxf(m[t], top), f = rescale(m[t], grown);
+                m[t] = grown;
+                l[t] *= f;
+#pragma unroll
+                for (int i = 0; i < F::NO; ++i) o[t][i] *= f;
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[t][j] = __builtin_amdgcn_exp2f(p[t][j] - base);
+                p[t][j] = __builtin_amdgcn_exp2f(p[t][j] - m[t]);
                 sum += p[t][j];
             }
-            l[t] = l[t] * f + sum;
-#pragma unroll
-            for (int i = 0; i < F::NO; ++i) o[t][i] *= f;
+            l[t] += sum;
         }
 
-        // O^T += V^T P^T
+        // O^T += V^T P^T; what is not admitted may hold anything: P = 0 meets V = 0
+        if (mask != 0xffffffffu) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vr[j] = (mine >> j) & 1 ? vr[j] : typename F::VRow{};
+        }
         if constexpr (F::MATH32) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -391,6 +406,7 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
                     for (int t = 0; t < NQ; ++t) o[t][i] = mfma16<F::F16>(vf, pf[t][term], o[t][i]);
             }
         }
+        if (more) load_v(c0 + 32 * FEW_WAVES);
     }
 
     // join the waves
@@ -450,11 +466,7 @@ template <int QT, int KVT, int DP, int NQ> __global__ __launch_bounds__(64 * FEW
 // (four keys of one column a lane) and P^T straight from the accumulators, rounded once to the products' type.
 // The 16-byte chunks of a row are permuted by its number (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4), by pairs of rows where rows are half
 // as long): both kinds of read then meet every bank evenly.  Rows of 16-bit values as long as the tile go from memory to LDS directly.
-// The maximum is only followed when it grows by more than 2^8: P is at most 256 then, its rounding is relative as before, and nearly all tiles skip
-// the rescaling of the sums.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;
-constexpr float MANY_SLACK = 8.0f;
-constexpr float MANY_NONE = -3.0e38f;        // maximum of a row that has seen no key: finite, so that no difference with it is NaN
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -471,7 +483,7 @@ __device__ inline u32x2 lds_read_transposed(const char* p)
 }
 // 16 bytes a lane from memory to LDS, the wave's 1024 in lane order from `lds` on; done when the wave has waited for its memory operations.  (The
 // builtin would have every later LDS read wait for it, as the compiler cannot tell the buffers apart.)
-__device__ inline void load_to_lds(const char* p, char* lds)
+__device__ inline void load_to_lds(mem p, char* lds)
 {
     const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory");
@@ -531,11 +543,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         if (a.c < 0) qf[u] ^= 0x80008000u;
     }
     const int lim = a.causal ? len - a.tq + rc / a.group + 1 : len;                 // this lane's row sees keys below it
-    int wave_lim = len, wave_first = len;                                             // the most and the fewest keys a row of this wave sees
-    if (a.causal) {
-        wave_first = len - a.tq + min(row0 + 32 * wave, a.rows - 1) / a.group + 1;
-        wave_lim = len - a.tq + min(row0 + 32 * wave + 31, a.rows - 1) / a.group + 1;
-    }
+    const int wave_first = a.causal ? len - a.tq + min(row0 + 32 * wave, a.rows - 1) / a.group + 1 : len;      // every row of this wave sees keys below it
 
     const char* kb = a.k + (int64_t)b * a.k_stride[0] + (int64_t)h * a.k_stride[2];
     const char* vb = a.v + (int64_t)b * a.v_stride[0] + (int64_t)h * a.v_stride[2];
@@ -547,8 +555,8 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     const int my_row = tid / ROW_LOADS, my_load = tid % ROW_LOADS;
     const int k_at = DIRECT ? (my_load ^ turn_k(my_row)) * 16 : my_load * 16, v_at = DIRECT ? (my_load ^ turn_v(my_row)) * 16 : my_load * 16;
     const bool in = FULL || my_load * 16 < a.d * (CODES ? 1 : 2);
-    const char* kp = kb + (uint64_t)my_row * (uint64_t)a.k_stride[1] + (in ? k_at : 0);
-    const char* vp = vb + (uint64_t)my_row * (uint64_t)a.v_stride[1] + (in ? v_at : 0);
+    const mem kp = (mem)(kb + (uint64_t)my_row * (uint64_t)a.k_stride[1] + (in ? k_at : 0));
+    const mem vp = (mem)(vb + (uint64_t)my_row * (uint64_t)a.v_stride[1] + (in ? v_at : 0));
 
     const int64_t k_step = LOAD_ROWS * a.k_stride[1], v_step = LOAD_ROWS * a.v_stride[1];
 
@@ -561,7 +569,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         return (uint64_t)__ballot(key < len && (!pad || pad[key] == 0));
     };
     // where this thread's loads of tile t of K or V come from (p: its first row's place in that tile); keys past the end are read from the last one
-    const auto aim = [&](int t, const char* p, int64_t stride, int64_t step, const char* (&x)[LOADS]) __attribute__((always_inline)) {
+    const auto aim = [&](int t, mem p, int64_t stride, int64_t step, mem (&x)[LOADS]) __attribute__((always_inline)) {
         const int c0 = t * MANY_KEYS;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) x[u] = u ? x[u - 1] + step : p;
@@ -572,9 +580,9 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         }
     };
     // ... load u of them, to registers or LDS
-    const auto load = [&](const char* const (&x)[LOADS], int u, u32x4* regs, char* lds) __attribute__((always_inline)) {
+    const auto load = [&](const mem (&x)[LOADS], int u, u32x4* regs, char* lds) __attribute__((always_inline)) {
         if constexpr (DIRECT) load_to_lds(x[u], lds + (u * MANY_WAVES + wave) * 1024);
-        else regs[u] = *reinterpret_cast<const u32x4*>(x[u]);
+        else regs[u] = load_as<u32x4>(x[u]);
     };
     // fetched registers into LDS (the caller waits and meets the other waves afterwards)
     const auto put = [&](u32x4* regs, char* lds, float scale, auto turn) __attribute__((always_inline)) {
@@ -628,7 +636,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     f32x16 o[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
-    float m = MANY_NONE, l = 0.0f;
+    float m = NO_MAX, l = 0.0f;
     uint64_t mask = 0;
     constexpr int AHEAD = 4, N = DP / 16, PAIRS = 8 / N;                             // N products of a half's scores, and of its output
     u32x4 kf[N];                                                                     // of the next half's scores, AHEAD of them read beforehand
@@ -648,7 +656,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     // soft-max and output of half `sub` of tile t from its scores s with their maximum `top`, and the scores of the half behind it: the matrix pipe
     // computes those while the exponentials run, and the output while their maximum is taken.  The next tiles' loads go out one at a time in between
     // (all at once they fill the memory pipe's queue and the wave waits: 1060 of 3500 cycles a tile).
-    const auto step = [&](int t, int sub, f32x16& s, float& top, const char* next_tile, const char* k_half_after, f32x16& next, const char* const (&from)[LOADS], u32x4* regs,
+    const auto step = [&](int t, int sub, f32x16& s, float& top, const char* next_tile, const char* k_half_after, f32x16& next, const mem (&from)[LOADS], u32x4* regs,
                           char* to) __attribute__((always_inline)) {
         const int c0 = t * MANY_KEYS + 32 * sub;
         const uint32_t bits = (uint32_t)(mask >> (32 * sub));
@@ -661,8 +669,8 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
             }
             top = most(s);
         }
-        if (__ballot(top > m + MANY_SLACK)) {
-            const float grown = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - grown);
+        if (__ballot(top > m + SLACK)) {
+            const float grown = fmaxf(m, top), f = rescale(m, grown);
             m = grown;
             l *= f;
 #pragma unroll
@@ -743,11 +751,11 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
 
     if (t0 < t1) {
         f32x16 sa, sb;
-        const char* from[LOADS];
+        mem from[LOADS];
         int now = 0, behind = 1, fetched = 2;                                           // K buffers of tiles t, t + 1, t + 2
         mask = admitted(t0);
         // this thread's first row of the tile that is loaded next
-        const char *k_from = kp + (int64_t)t0 * MANY_KEYS * a.k_stride[1], *v_from = vp + (int64_t)t0 * MANY_KEYS * a.v_stride[1];
+        mem k_from = kp + (int64_t)t0 * MANY_KEYS * a.k_stride[1], v_from = vp + (int64_t)t0 * MANY_KEYS * a.v_stride[1];
         const int64_t k_tile = MANY_KEYS * a.k_stride[1], v_tile = MANY_KEYS * a.v_stride[1];
         const auto bring_k = [&](int t, int buf) __attribute__((always_inline)) {
             aim(t, k_from, a.k_stride[1], k_step, from);
@@ -837,7 +845,7 @@ template <int QT> __global__ __launch_bounds__(256) void attention_join_kernel(A
         const int64_t row = e / per_row;
         const int r = (int)(row % a.rows), bh = (int)(row / a.rows), b = bh / a.kv_heads, h = bh % a.kv_heads;
         const float* ws = a.ws + row * (a.d + 4);
-        float top = NEG_INF;
+        float top = NO_MAX;
         for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, ws[s * split_stride]);
         float sum = 0.0f;
         f32x4 acc{};
@@ -898,8 +906,10 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
 template <int QT, int KVT> hipError_t launch_few(const AttnArgs& a, int nq, hipStream_t s)
 {
     const dim3 grid((uint32_t)((int64_t)a.n * a.kv_heads * a.nsplit * a.tiles)), block(64 * FEW_WAVES);
-    if (a.d <= 64) return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 64, 1>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 64, 2>, grid, block, s, a);
-    return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 128, 1>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 128, 2>, grid, block, s, a);
+    if (a.d == 64) return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 64, 1, true>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 64, 2, true>, grid, block, s, a);
+    if (a.d == 128) return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 128, 1, true>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 128, 2, true>, grid, block, s, a);
+    if (a.d < 64) return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 64, 1, false>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 64, 2, false>, grid, block, s, a);
+    return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 128, 1, false>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 128, 2, false>, grid, block, s, a);
 }
 
 template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, hipStream_t s)
