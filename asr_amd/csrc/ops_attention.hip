@@ -834,37 +834,53 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         }
 }
 
-// joins the shares of a long key axis: one thread per four output values
-template <int QT> __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a)
+// Joins the shares of a long key axis.  A row has 32 G threads: four values each, every G-th share (a row's shares are far apart, so the loads of many
+// have to be in flight: with one thread for all 64 shares of a row this took 35 us of a 50 us call), then the G sums in LDS.
+template <int QT, int G> __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a)
 {
-    const int per_row = a.d / 4;
-    const int64_t total = (int64_t)a.n * a.kv_heads * a.rows * per_row;
-    const int64_t split_stride = (int64_t)a.n * a.kv_heads * a.rows * (a.d + 4);
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int at = (int)(e % per_row) * 4;
-        const int64_t row = e / per_row;
-        const int r = (int)(row % a.rows), bh = (int)(row / a.rows), b = bh / a.kv_heads, h = bh % a.kv_heads;
+    constexpr int ROWS = 8 / G;
+    __shared__ __align__(16) float s_acc[ROWS][G][32][4];
+    __shared__ float s_sum[ROWS][G];
+    const int lane = threadIdx.x & 31, g = threadIdx.x / 32 % G, slot = threadIdx.x / (32 * G), at = 4 * lane;
+    const int64_t rows = (int64_t)a.n * a.kv_heads * a.rows, split_stride = rows * (a.d + 4);
+    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < rows; row0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = row0 + slot < rows ? row0 + slot : rows - 1;
         const float* ws = a.ws + row * (a.d + 4);
         float top = NO_MAX;
-        for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, ws[s * split_stride]);
+        for (int s = lane; s < a.nsplit; s += 32) top = fmaxf(top, ws[s * split_stride]);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 32));
         float sum = 0.0f;
         f32x4 acc{};
-        for (int s = 0; s < a.nsplit; ++s) {
+#pragma unroll 4
+        for (int s = g; s < a.nsplit; s += G) {
             const float* p = ws + s * split_stride;
             const float f = rescale(p[0], top);
             sum += p[1] * f;
-            acc += *reinterpret_cast<const f32x4*>(p + 4 + at) * f;
+            acc += *reinterpret_cast<const f32x4*>(p + 4 + (at < a.d ? at : 0)) * f;
         }
-        acc = sum == 0.0f ? f32x4{} : acc * (1.0f / sum);
-        char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] +
-                   (int64_t)(h * a.group + r % a.group) * a.out_stride[2] + at * (QT == ASR_F32 ? 4 : 2);
-        if constexpr (QT == ASR_F32) *reinterpret_cast<f32x4*>(op) = acc;
-        else {
-            u32x2 w;
-            w[0] = pack16<QT == ASR_F16>(acc[0], acc[1]);
-            w[1] = pack16<QT == ASR_F16>(acc[2], acc[3]);
-            *reinterpret_cast<u32x2*>(op) = w;
+        *reinterpret_cast<f32x4*>(s_acc[slot][g][lane]) = acc;
+        if (lane == 0) s_sum[slot][g] = sum;
+        __syncthreads();
+        if (g == 0 && at < a.d && row0 + slot < rows) {
+#pragma unroll
+            for (int i = 1; i < G; ++i) {
+                acc += *reinterpret_cast<const f32x4*>(s_acc[slot][i][lane]);
+                sum += s_sum[slot][i];
+            }
+            acc = sum == 0.0f ? f32x4{} : acc * (1.0f / sum);
+            const int r = (int)(row % a.rows), bh = (int)(row / a.rows), b = bh / a.kv_heads, h = bh % a.kv_heads;
+            char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] +
+                       (int64_t)(h * a.group + r % a.group) * a.out_stride[2] + at * (QT == ASR_F32 ? 4 : 2);
+            if constexpr (QT == ASR_F32) *reinterpret_cast<f32x4*>(op) = acc;
+            else {
+                u32x2 w;
+                w[0] = pack16<QT == ASR_F16>(acc[0], acc[1]);
+                w[1] = pack16<QT == ASR_F16>(acc[2], acc[3]);
+                *reinterpret_cast<u32x2*>(op) = w;
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -893,9 +909,10 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
     }
     p.nq = p.rows > 16 ? 2 : 1;
     p.tiles = (p.rows + 16 * p.nq - 1) / (16 * p.nq);
-    // shares of the key axis: enough workgroups for the chip (two for each of 256 compute units), each with at least four chunks of 32 keys for each wave
+    // shares of the key axis: enough workgroups for the chip (three for each of 256 compute units: 16 x 4 queries over 4096 f32 keys 41 us with one, 31 with
+    // two, 29 with three), each with at least four chunks of 32 keys for each wave
     const int64_t wgs = n * kv_heads * p.tiles, most = tk / (FEW_WAVES * 32 * 4);
-    int64_t split = wgs > 0 ? (512 + wgs - 1) / wgs : 1;
+    int64_t split = wgs > 0 ? (768 + wgs - 1) / wgs : 1;
     if (split > most) split = most;
     if (split > 64) split = 64;
     p.nsplit = split < 1 ? 1 : (int)split;
@@ -922,8 +939,9 @@ template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, hipStream_t
 
 template <int QT> hipError_t launch_join(const AttnArgs& a, hipStream_t s)
 {
-    const int64_t blocks = ((int64_t)a.n * a.kv_heads * a.rows * (a.d / 4) + 255) / 256;
-    return ops_launch(attention_join_kernel<QT>, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), s, a);
+    const int64_t rows = (int64_t)a.n * a.kv_heads * a.rows, blocks = a.nsplit >= 8 ? rows : (rows + 3) / 4;
+    const dim3 grid((uint32_t)(blocks < 65536 ? blocks : 65536)), block(256);
+    return a.nsplit >= 8 ? ops_launch(attention_join_kernel<QT, 8>, grid, block, s, a) : ops_launch(attention_join_kernel<QT, 2>, grid, block, s, a);
 }
 
 template <int QT, int KVT> int attend(const char* what, AttnArgs& a, const Plan& p, void* ws, int64_t ws_bytes, hipStream_t s)

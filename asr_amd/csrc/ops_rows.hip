@@ -371,10 +371,9 @@ namespace {
 // ---- kv8_append --------------------------------------------------------------------------------------------------------
 // One workgroup per (64-token block that may get tokens, sequence and head, K or V): the new tokens' magnitudes -> the block's
 // exponent -> codes.  The scale is 2^e with the smallest e that keeps the magnitudes within 448 = 1.75 * 2^8, found in the bits of the largest one;
-// dividing by a power of two is exact, so a value is rounded once.  Moving bytes bounds it: each new value is read once (the second reading, for the
-// codes, comes from registers or the cache), each code written once.
+// dividing by a power of two is exact, so a value is rounded once.  Moving bytes bounds it: each new value is read once, into registers, each code written
+// once.  Neighbouring workgroups take the heads of the same tokens, which lie side by side in the projection's output.
 constexpr int KV8_MIN_EXP = -100;
-constexpr int KV8_THREADS = 256;
 
 __device__ inline int kv8_exponent(uint32_t magnitude)          // of a finite float's bits without sign
 {
@@ -402,50 +401,59 @@ struct Kv8AppendArgs {
     int new_tokens, kv_heads, d, capacity;
 };
 
-template <int DT> __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kernel(Kv8AppendArgs a)
+// NT threads, each with up to ITEMS 16-byte loads of the block's new tokens
+template <int DT, int NT, int ITEMS> __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8AppendArgs a)
 {
     typedef typename Elem<DT>::T T;
-    constexpr int PER = Elem<DT>::PER;
-    __shared__ uint32_t top_bits[KV8_THREADS / 64];
-    const int which = blockIdx.z & 1, b = blockIdx.z >> 1, h = blockIdx.y;
+    constexpr int PER = Elem<DT>::PER, NW = NT / 64;
+    __shared__ uint32_t top_bits[NW];
+    const int which = (int)blockIdx.x >= a.kv_heads, h = blockIdx.x - (which ? a.kv_heads : 0), b = blockIdx.z;
     const int held = a.lens[b];
     if (held < 0 || held >= a.capacity) return;
     const int count = a.counts ? min(a.counts[b], a.new_tokens) : a.new_tokens;
     const int end = (int)min((int64_t)a.capacity, (int64_t)held + count);        // positions held .. end get tokens
-    const int block = held / ASR_KV8_BLOCK + blockIdx.x, first = block * ASR_KV8_BLOCK;
+    const int block = held / ASR_KV8_BLOCK + blockIdx.y, first = block * ASR_KV8_BLOCK;
     const int lo = max(held, first), hi = min(end, first + ASR_KV8_BLOCK);
-    if (lo >= hi) return;
+    if (block >= a.capacity / ASR_KV8_BLOCK || lo >= hi) return;
     const int tid = threadIdx.x, per_row = a.d / PER, items = (hi - lo) * per_row;
-    const T* x = static_cast<const T*>(a.x[which]) + (int64_t)b * a.stride[which][0] + (int64_t)h * a.stride[which][2];
+    const T* x = static_cast<const T*>(a.x[which]) + (int64_t)b * a.stride[which][0] + (int64_t)h * a.stride[which][2] + (int64_t)(lo - held) * a.stride[which][1];
     uint8_t* codes = a.cache[which] + (int64_t)b * a.cache_stride[0] + (int64_t)h * a.cache_stride[1] + (int64_t)first * a.d;
     float* scale = a.scale[which] + ((int64_t)b * a.kv_heads + h) * (a.capacity / ASR_KV8_BLOCK) + block;
+    const float was = *scale;
 
+    u32x4 raw[ITEMS];
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+        const int i = tid + u * NT, t = i / per_row, c = i - t * per_row;
+        raw[u] = i < items ? *reinterpret_cast<const u32x4*>(x + (int64_t)t * a.stride[which][1] + c * PER) : u32x4{};
+    }
     uint32_t most = 0;
-    for (int i = tid; i < items; i += KV8_THREADS) {
-        const int t = i / per_row, c = i % per_row;
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
         float y[PER];
-        Elem<DT>::unpack(*reinterpret_cast<const u32x4*>(x + (int64_t)(lo - held + t) * a.stride[which][1] + c * PER), y);
+        Elem<DT>::unpack(raw[u], y);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const uint32_t u = __float_as_uint(y[j]) & 0x7fffffffu;
-            if (u < 0x7f800000u) most = max(most, u);
+            const uint32_t m = __float_as_uint(y[j]) & 0x7fffffffu;
+            most = max(most, m < 0x7f800000u ? m : 0u);
         }
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-    if ((tid & 63) == 0) top_bits[tid >> 6] = most;
-    __syncthreads();
+    if (NW > 1) {
+        if ((tid & 63) == 0) top_bits[tid >> 6] = most;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < KV8_THREADS / 64; ++i) most = max(most, top_bits[i]);
+        for (int i = 0; i < NW; ++i) most = max(most, top_bits[i]);
+    }
     int e = kv8_exponent(most);
     if (held > first) {                                              // the block holds older tokens: its scale only grows
-        const float was = *scale;
         const int e_was = min(max((int)(__float_as_uint(was) >> 23) - 127, KV8_MIN_EXP), 120);
         if (e > e_was) {
             // the older tokens under the new scale (a power of two lower: exact unless a code becomes subnormal)
             const float f = pow2f(max(e_was - e, -126));
             uint32_t* old = reinterpret_cast<uint32_t*>(codes);
-            for (int i = tid; i < (held - first) * a.d / 4; i += KV8_THREADS) {
+            for (int i = tid; i < (held - first) * a.d / 4; i += NT) {
                 const uint32_t c = old[i];
                 typedef float f32x2 __attribute__((ext_vector_type(2)));
                 const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
@@ -455,17 +463,30 @@ template <int DT> __global__ __launch_bounds__(KV8_THREADS) void kv8_append_kern
         e = max(e, e_was);
     }
     const float inv = pow2f(-e);
-    for (int i = tid; i < items; i += KV8_THREADS) {
-        const int t = i / per_row, c = i % per_row;
-        float y[PER];
-        Elem<DT>::unpack(*reinterpret_cast<const u32x4*>(x + (int64_t)(lo - held + t) * a.stride[which][1] + c * PER), y);
-        uint32_t* out = reinterpret_cast<uint32_t*>(codes + (int64_t)(lo - first + t) * a.d + c * PER);
+    uint8_t* to = codes + (lo - first) * a.d;
 #pragma unroll
-        for (int j = 0; j < PER / 4; ++j)
-            out[j] = kv8_codes(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
+    for (int u = 0; u < ITEMS; ++u) {
+        const int i = tid + u * NT;                                  // (the new tokens' codes are dense)
+        if (i >= items) continue;
+        float y[PER];
+        Elem<DT>::unpack(raw[u], y);
+        uint32_t w[PER / 4];
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) w[j] = kv8_codes(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
+        uint32_t* out = reinterpret_cast<uint32_t*>(to + i * PER);
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) out[j] = w[j];
     }
-    __syncthreads();                                                 // (every thread has read the old scale)
-    if (tid == 0) *scale = pow2f(e);
+    if (tid == 0) *scale = pow2f(e);                                 // (every thread of a wider workgroup has read the old one: the barrier above)
+}
+
+template <int DT> hipError_t run_kv8_append(const Kv8AppendArgs& k, dim3 grid, hipStream_t s)
+{
+    constexpr int PER = Elem<DT>::PER;
+    // a few tokens: one wave holds a block's share (64 sequences, one token, 16 heads: 4.7 us with four waves)
+    if (k.new_tokens * k.d <= 64 * PER) return ops_launch(kv8_append_kernel<DT, 64, 1>, grid, dim3(64), s, k);
+    if (k.d <= 64) return ops_launch(kv8_append_kernel<DT, 256, 64 * 64 / PER / 256>, grid, dim3(256), s, k);
+    return ops_launch(kv8_append_kernel<DT, 256, 64 * 128 / PER / 256>, grid, dim3(256), s, k);
 }
 
 }  // namespace
@@ -493,7 +514,8 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream)
         return ops_fail(ASR_ERR_ARG, "kv8_append: rows of k and v must start on 16 bytes");
     if (((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) || a->cache_stride[0] % 16 || a->cache_stride[1] % 16)
         return ops_fail(ASR_ERR_ARG, "kv8_append: cache rows must start on 16 bytes");
-    if (a->n > 32767 || a->kv_heads > 65535) return ops_fail(ASR_ERR_ARG, "kv8_append: at most 32767 sequences and 65535 heads a call");
+    if (a->n > 65535 || a->kv_heads > (1 << 20) || (int64_t)a->new_tokens > 65000 * (int64_t)ASR_KV8_BLOCK)
+        return ops_fail(ASR_ERR_ARG, "kv8_append: at most 65535 sequences, 2^20 heads and 65000 blocks of tokens a call");
     Kv8AppendArgs k{};
     k.x[0] = a->k; k.x[1] = a->v;
     k.cache[0] = a->k_cache; k.cache[1] = a->v_cache;
@@ -505,11 +527,10 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream)
     // blocks that new_tokens tokens can touch, wherever the first one falls
     const int64_t touched = ((int64_t)a->new_tokens + ASR_KV8_BLOCK - 2) / ASR_KV8_BLOCK + 1;
     const int blocks = (int)(touched < a->capacity / ASR_KV8_BLOCK ? touched : a->capacity / ASR_KV8_BLOCK);
-    const dim3 grid(blocks, a->kv_heads, 2 * a->n);
+    const dim3 grid(2 * a->kv_heads, blocks, a->n);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return ops_launched("kv8_append", a->dtype == ASR_F32 ? ops_launch(kv8_append_kernel<ASR_F32>, grid, dim3(KV8_THREADS), s, k)
-                                      : a->dtype == ASR_BF16 ? ops_launch(kv8_append_kernel<ASR_BF16>, grid, dim3(KV8_THREADS), s, k)
-                                                             : ops_launch(kv8_append_kernel<ASR_F16>, grid, dim3(KV8_THREADS), s, k));
+    return ops_launched("kv8_append", a->dtype == ASR_F32 ? run_kv8_append<ASR_F32>(k, grid, s)
+                                      : a->dtype == ASR_BF16 ? run_kv8_append<ASR_BF16>(k, grid, s) : run_kv8_append<ASR_F16>(k, grid, s));
 }
 
 }  // extern "C"
