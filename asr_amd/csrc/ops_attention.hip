@@ -132,10 +132,13 @@ __device__ inline int place_of(int nbh, int per, int64_t& id)
 // tile: bound by those bytes while there are few rows.  QT: type of q and out, KVT: of K and V.
 // Terms: 16-bit K / V are exact factors; q enters as QTERMS 16-bit terms (bf16 codes: f16 = 2, f32 = 3 bf16 terms lose nothing) and
 // P as PTERMS (two: 2^-17 / 2^-22 of it lost, three: nothing), which costs matrix instructions that a loop waiting for memory has to spare.
+// float32 K / V are cut into three bf16 terms as well (8 + 8 + 8 bits: exact), and of the nine products the six above 2^-24 are taken: the 16-bit matrix
+// pipe is 16 times the float32 one, which besides shares its units with the vector instructions (50 x 61 queries over 1000 states of 16 heads:
+// 133 us on the float32 instruction).
 template <int QT, int KVT, int DP, int NQ> struct Few {
     static constexpr bool MATH32 = KVT == KV_F32, F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
-    static constexpr int QTERMS = CODES ? (QT == ASR_F32 ? 3 : QT == ASR_F16 ? 2 : 1) : 1;
-    static constexpr int PTERMS = CODES && QT == ASR_F32 ? 3 : 2;
+    static constexpr int QTERMS = QT == ASR_F32 ? 3 : CODES && QT == ASR_F16 ? 2 : 1;
+    static constexpr int PTERMS = QT == ASR_F32 ? 3 : 2, KTERMS = MATH32 ? 3 : 1;
     static constexpr int KVB = KVT == KV_F32 ? 4 : CODES ? 1 : 2;         // bytes of a K / V value
     static constexpr int QB = QT == ASR_F32 ? 4 : 2;
     static constexpr int KW = DP / 4 * KVB / 4;                             // words of a key row in one lane (a quarter of it)
@@ -145,6 +148,32 @@ template <int QT, int KVT, int DP, int NQ> struct Few {
 };
 
 constexpr int FEW_WAVES = 4;
+
+// eight float32 values as three bf16 vectors that add up to them: the upper half of each, of what is left, and of what is left then (exact; an infinite value
+// leaves NaN)
+__device__ inline void cut(const uint32_t (&x)[8], u32x4 (&t)[3])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t a = x[2 * j], b = x[2 * j + 1];
+        const float a1 = __uint_as_float(a) - __uint_as_float(a & 0xffff0000u), b1 = __uint_as_float(b) - __uint_as_float(b & 0xffff0000u);
+        const uint32_t a1u = __float_as_uint(a1), b1u = __float_as_uint(b1);
+        const float a2 = a1 - __uint_as_float(a1u & 0xffff0000u), b2 = b1 - __uint_as_float(b1u & 0xffff0000u);
+        t[0][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        t[1][j] = __builtin_amdgcn_perm(b1u, a1u, 0x07060302u);
+        t[2][j] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a2), 0x07060302u);
+    }
+}
+// c + a b over bf16 terms of a and b, those above 2^-24 of the product, the smallest first
+template <bool F16, int NA, int NB> __device__ inline f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c)
+{
+#pragma unroll
+    for (int sum = NA + NB - 2 < 2 ? NA + NB - 2 : 2; sum >= 0; --sum)
+#pragma unroll
+        for (int i = NA - 1; i >= 0; --i)
+            if (sum - i >= 0 && sum - i < NB) c = mfma16<F16>(a[i], b[sum - i], c);
+    return c;
+}
 
 // the place in a row of value j (0 .. DP/4) of lane group g's quarter of it
 template <int KVT> __device__ constexpr int quarter_at(int g, int j)
@@ -172,48 +201,32 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
     const int chunk0 = split * share, chunk1 = min(chunks, chunk0 + share);
 
     // q in the second operand's layout: lane x16 holds row x16, lane group g its quarter of the row
-    u32x4 qf[NQ][F::QTERMS][F::MATH32 ? DP / 16 : DP / 32];
+    u32x4 qf[NQ][DP / 32][F::QTERMS];
     int lim[NQ];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
         const int r = row0 + 16 * t + x16, rc = min(r, a.rows - 1);
         lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
         const char* qp = a.q + (int64_t)b * a.q_stride[0] + (int64_t)(rc / a.group) * a.q_stride[1] + (int64_t)(h * a.group + rc % a.group) * a.q_stride[2];
-        if constexpr (F::MATH32) {
 #pragma unroll
-            for (int u = 0; u < DP / 16; ++u) {
-                const int at = quarter_at<KVT>(g, 4 * u);
-                qf[t][0][u] = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 4 * at) : u32x4{};
-            }
-        } else {
+        for (int u = 0; u < DP / 32; ++u) {
+            // eight values: consecutive, or (float32 K) four and four
+            const int at = quarter_at<KVT>(g, 8 * u), at2 = quarter_at<KVT>(g, 8 * u + 4);
+            const bool in = at < a.d && r < a.rows, in2 = at2 < a.d && r < a.rows;
+            if constexpr (F::QTERMS == 1) qf[t][u][0] = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
+            else if constexpr (QT == ASR_F32) {
+                const u32x4 lo = in ? *reinterpret_cast<const u32x4*>(qp + 4 * at) : u32x4{}, hi = in2 ? *reinterpret_cast<const u32x4*>(qp + 4 * at2) : u32x4{};
+                const uint32_t x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                cut(x, qf[t][u]);
+            } else {
+                const u32x4 w = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
 #pragma unroll
-            for (int u = 0; u < DP / 32; ++u) {
-                const int at = quarter_at<KVT>(g, 8 * u);                  // eight consecutive values
-                const bool in = at < a.d && r < a.rows;
-                if constexpr (F::QTERMS == 1) qf[t][0][u] = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
-                else {
-                    float x[8];
-                    if constexpr (QT == ASR_F32) {
-                        const f32x4 p = in ? *reinterpret_cast<const f32x4*>(qp + 4 * at) : f32x4{};
-                        const f32x4 p2 = in ? *reinterpret_cast<const f32x4*>(qp + 4 * at + 16) : f32x4{};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { x[j] = p[j]; x[4 + j] = p2[j]; }
-                    } else {
-                        const u32x4 p = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { const f32x2 y = unpack16<true>(p[j]); x[2 * j] = y[0]; x[2 * j + 1] = y[1]; }
-                    }
-#pragma unroll
-                    for (int term = 0; term < F::QTERMS; ++term)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t w = pack_bf16(x[2 * j], x[2 * j + 1]);
-                            qf[t][term][u][j] = w;
-                            const f32x2 y = unpack16<false>(w);
-                            // an infinite value has no rest (inf - inf would make NaN of it)
-                            x[2 * j] = __builtin_isinf(y[0]) ? 0.0f : x[2 * j] - y[0];
-                            x[2 * j + 1] = __builtin_isinf(y[1]) ? 0.0f : x[2 * j + 1] - y[1];
-                        }
+                for (int j = 0; j < 4; ++j) {
+                    const f32x2 y = unpack16<true>(w[j]);
+                    const uint32_t hi = pack_bf16(y[0], y[1]);
+                    const f32x2 z = unpack16<false>(hi);
+                    qf[t][u][0][j] = hi;
+                    qf[t][u][1][j] = pack_bf16(y[0] - z[0], y[1] - z[1]);
                 }
             }
         }
@@ -307,28 +320,21 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
         for (int t = 0; t < NQ; ++t) s[t][0] = s[t][1] = f32x4{};
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
-            if constexpr (F::MATH32) {
 #pragma unroll
-                for (int w = 0; w < F::KW; ++w)
+            for (int u = 0; u < DP / 32; ++u) {
+                u32x4 kf[F::KTERMS];
+                if constexpr (F::MATH32) {
+                    const u32x4 &lo = kr[t2][2 * u], &hi = kr[t2][2 * u + 1];
+                    const uint32_t x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    cut(x, kf);
+                } else if constexpr (F::CODES) {
+                    const uint32_t lo = kr[t2][u / 2][2 * (u & 1)], hi = kr[t2][u / 2][2 * (u & 1) + 1];
+                    kf[0] = u32x4{codes_bf16<false>(lo, ks), codes_bf16<true>(lo, ks), codes_bf16<false>(hi, ks), codes_bf16<true>(hi, ks)};
+                } else kf[0] = kr[t2][u];
 #pragma unroll
-                    for (int t = 0; t < NQ; ++t)
-                        s[t][t2] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t2][w / 4][w % 4]), __uint_as_float(qf[t][0][w / 4][w % 4]), s[t][t2], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int u = 0; u < DP / 32; ++u) {
-                    u32x4 kf;
-                    if constexpr (F::CODES) {
-                        const uint32_t lo = kr[t2][u / 2][2 * (u & 1)], hi = kr[t2][u / 2][2 * (u & 1) + 1];
-                        kf = u32x4{codes_bf16<false>(lo, ks), codes_bf16<true>(lo, ks), codes_bf16<false>(hi, ks), codes_bf16<true>(hi, ks)};
-                    } else kf = kr[t2][u];
-#pragma unroll
-                    for (int term = F::QTERMS - 1; term >= 0; --term)
-#pragma unroll
-                        for (int t = 0; t < NQ; ++t) s[t][t2] = mfma16<F::F16>(kf, qf[t][term][u], s[t][t2]);
-                }
+                for (int t = 0; t < NQ; ++t) s[t][t2] = mfma_terms<F::F16>(kf, qf[t][u], s[t][t2]);
             }
         }
-
         if (more) load_k(c0 + 32 * FEW_WAVES);
 
         // soft-max step; p[t][4 t2 + i] belongs to key 8 g + 4 t2 + i
@@ -367,44 +373,38 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
 #pragma unroll
             for (int j = 0; j < 8; ++j) vr[j] = (mine >> j) & 1 ? vr[j] : typename F::VRow{};
         }
-        if constexpr (F::MATH32) {
+        u32x4 pf[NQ][F::PTERMS];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
-                for (int w = 0; w < F::VW; ++w)
+            for (int term = 0; term < F::PTERMS; ++term)
 #pragma unroll
-                    for (int t = 0; t < NQ; ++t) o[t][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][w]), p[t][j], o[t][w], 0, 0, 0);
-        } else {
-            u32x4 pf[NQ][F::PTERMS];
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = pack16<F::F16>(p[t][2 * j], p[t][2 * j + 1]);
+                    pf[t][term][j] = w;
+                    const f32x2 y = unpack16<F::F16>(w);
+                    p[t][2 * j] -= y[0];
+                    p[t][2 * j + 1] -= y[1];
+                }
 #pragma unroll
-            for (int t = 0; t < NQ; ++t)
-#pragma unroll
-                for (int term = 0; term < F::PTERMS; ++term)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t w = pack16<F::F16>(p[t][2 * j], p[t][2 * j + 1]);
-                        pf[t][term][j] = w;
-                        const f32x2 y = unpack16<F::F16>(w);
-                        p[t][2 * j] -= y[0];
-                        p[t][2 * j + 1] -= y[1];
-                    }
-#pragma unroll
-            for (int i = 0; i < F::NO; ++i) {
-                u32x4 vf;
+        for (int i = 0; i < F::NO; ++i) {
+            u32x4 vf[F::KTERMS];
+            if constexpr (F::MATH32) {
+                const uint32_t x[8] = {vr[0][i], vr[1][i], vr[2][i], vr[3][i], vr[4][i], vr[5][i], vr[6][i], vr[7][i]};
+                cut(x, vf);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if constexpr (F::CODES) {
                         const uint32_t two = __builtin_amdgcn_perm(vr[2 * j + 1][i >> 2], vr[2 * j][i >> 2], i & 2 ? 0x07030602u : 0x05010400u);
-                        vf[j] = i & 1 ? codes_bf16<true>(two, vs) : codes_bf16<false>(two, vs);
+                        vf[0][j] = i & 1 ? codes_bf16<true>(two, vs) : codes_bf16<false>(two, vs);
                     } else {
-                        vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][i >> 1], vr[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+                        vf[0][j] = __builtin_amdgcn_perm(vr[2 * j + 1][i >> 1], vr[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
                     }
                 }
-#pragma unroll
-                for (int term = F::PTERMS - 1; term >= 0; --term)
-#pragma unroll
-                    for (int t = 0; t < NQ; ++t) o[t][i] = mfma16<F::F16>(vf, pf[t][term], o[t][i]);
             }
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) o[t][i] = mfma_terms<F::F16>(vf, pf[t], o[t][i]);
         }
         if (more) load_v(c0 + 32 * FEW_WAVES);
     }
