@@ -181,7 +181,9 @@ template <int KVT> __device__ constexpr int quarter_at(int g, int j)
     return KVT == KV_F32 ? 16 * (j >> 2) + 4 * g + (j & 3) : KVT == KV_E4M3 ? 64 * (j >> 4) + 16 * g + (j & 15) : 32 * (j >> 3) + 8 * g + (j & 7);
 }
 
-template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds__(64 * FEW_WAVES) void attention_few_kernel(AttnArgs a)
+// (two workgroups on a compute unit but where float32 rows of 128 need all registers)
+template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds__(64 * FEW_WAVES, KVT == KV_F32 && DP == 128 && NQ == 2 ? 1 : 2)
+void attention_few_kernel(AttnArgs a)
 {
     typedef Few<QT, KVT, DP, NQ> F;
     constexpr int PITCH = DP + 4;
@@ -231,6 +233,8 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
             }
         }
     }
+
+    const int first_lim = a.causal ? len - a.tq + row0 / a.group + 1 : 0x7fffffff;       // every row of this tile sees the keys below it
 
     f32x4 o[NQ][F::NO];
     float m[NQ], l[NQ];
@@ -313,7 +317,6 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
         const bool more = chunk + FEW_WAVES < chunk1;
         // one admitted-bit per key of the chunk, the same for the whole wave
         const uint32_t mask = (uint32_t)__ballot(c0 + (lane & 31) < len && flag == 0);
-        const uint32_t mine = mask >> (8 * g);                                 // bits 0 .. 7: keys 8 g .. 8 g + 7
         // S^T
         f32x4 s[NQ][2];
 #pragma unroll
@@ -343,10 +346,15 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
         for (int t = 0; t < NQ; ++t) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[t][j] = s[t][j >> 2][j & 3] * a.c;
-            if (mask != 0xffffffffu || a.causal) {
+            if (mask != 0xffffffffu) {
+                asm volatile("");                                              // (a branch, not selects in every chunk)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[t][j] = (mask >> (8 * g + j)) & 1 ? p[t][j] : NEG_INF;
+            }
+            if (c0 + 32 > first_lim) {                                         // (causal calls)
                 asm volatile("");
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[t][j] = ((mine >> j) & 1) && c0 + 8 * g + j < lim[t] ? p[t][j] : NEG_INF;
+                for (int j = 0; j < 8; ++j) p[t][j] = c0 + 8 * g + j < lim[t] ? p[t][j] : NEG_INF;
             }
             float top = p[t][0];
 #pragma unroll
@@ -371,7 +379,7 @@ template <int QT, int KVT, int DP, int NQ, bool FULL> __global__ __launch_bounds
         // O^T += V^T P^T; what is not admitted may hold anything: P = 0 meets V = 0
         if (mask != 0xffffffffu) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) vr[j] = (mine >> j) & 1 ? vr[j] : typename F::VRow{};
+            for (int j = 0; j < 8; ++j) vr[j] = (mask >> (8 * g + j)) & 1 ? vr[j] : typename F::VRow{};
         }
         u32x4 pf[NQ][F::PTERMS];
 #pragma unroll
