@@ -84,6 +84,10 @@ template <bool HI> __device__ inline uint32_t codes_bf16(uint32_t w, float scale
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, HI));
 }
 
+// all ones where bit `at` of `bits` is set; x there, else -infinity (two instructions a value)
+__device__ inline uint32_t spread_bit(uint32_t bits, int at) { return (uint32_t)((int32_t)(bits << (31 - at)) >> 31); }
+__device__ inline float admit(float x, uint32_t ones) { return __uint_as_float((__float_as_uint(x) & ones) | (0xff800000u & ~ones)); }
+
 // maximum / sum over the four 16-lane groups of a wave
 __device__ inline float groups_max(float x)
 {
@@ -317,6 +321,7 @@ void attention_few_kernel(AttnArgs a)
         const bool more = chunk + FEW_WAVES < chunk1;
         // one admitted-bit per key of the chunk, the same for the whole wave
         const uint32_t mask = (uint32_t)__ballot(c0 + (lane & 31) < len && flag == 0);
+        const uint32_t mine = mask >> (8 * g);                                 // bits 0 .. 7: keys 8 g .. 8 g + 7
         // S^T
         f32x4 s[NQ][2];
 #pragma unroll
@@ -349,7 +354,7 @@ void attention_few_kernel(AttnArgs a)
             if (mask != 0xffffffffu) {
                 asm volatile("");                                              // (a branch, not selects in every chunk)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[t][j] = (mask >> (8 * g + j)) & 1 ? p[t][j] : NEG_INF;
+                for (int j = 0; j < 8; ++j) p[t][j] = admit(p[t][j], spread_bit(mine, j));
             }
             if (c0 + 32 > first_lim) {                                         // (causal calls)
                 asm volatile("");
@@ -379,7 +384,7 @@ void attention_few_kernel(AttnArgs a)
         // O^T += V^T P^T; what is not admitted may hold anything: P = 0 meets V = 0
         if (mask != 0xffffffffu) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) vr[j] = (mask >> (8 * g + j)) & 1 ? vr[j] : typename F::VRow{};
+            for (int j = 0; j < 8; ++j) vr[j] &= spread_bit(mine, j);
         }
         u32x4 pf[NQ][F::PTERMS];
 #pragma unroll
@@ -551,7 +556,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         if (a.c < 0) qf[u] ^= 0x80008000u;
     }
     const int lim = a.causal ? len - a.tq + rc / a.group + 1 : len;                 // this lane's row sees keys below it
-    const int wave_first = a.causal ? len - a.tq + min(row0 + 32 * wave, a.rows - 1) / a.group + 1 : len;      // every row of this wave sees keys below it
+    const int wave_first = a.causal ? len - a.tq + min(row0 + 32 * wave, a.rows - 1) / a.group + 1 : 0x7fffffff;      // every row of this wave sees keys below it
 
     const char* kb = a.k + (int64_t)b * a.k_stride[0] + (int64_t)h * a.k_stride[2];
     const char* vb = a.v + (int64_t)b * a.v_stride[0] + (int64_t)h * a.v_stride[2];
@@ -570,11 +575,14 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
 
     u32x4 kr[DIRECT ? 1 : LOADS], vr[DIRECT ? 1 : LOADS];
     float ks = 1.0f, vs = 1.0f;
-    // one bit for each admitted key of tile t
-    const auto admitted = [&](int t) __attribute__((always_inline)) {
-        if (!pad && (t + 1) * MANY_KEYS <= len) return ~(uint64_t)0;
+    // one bit for each admitted key of tile t, from this lane's flag of it (asked for a tile ahead: waiting for it costs as much as half a tile)
+    const auto flag_of = [&](int t) __attribute__((always_inline)) {
         const int key = t * MANY_KEYS + lane;
-        return (uint64_t)__ballot(key < len && (!pad || pad[key] == 0));
+        return pad && key < len ? (uint32_t)pad[key] : 0u;
+    };
+    const auto admitted = [&](int t, uint32_t flag) __attribute__((always_inline)) {
+        if (!pad && (t + 1) * MANY_KEYS <= len) return ~(uint64_t)0;
+        return (uint64_t)__ballot(t * MANY_KEYS + lane < len && flag == 0);
     };
     // where this thread's loads of tile t of K or V come from (p: its first row's place in that tile); keys past the end are read from the last one
     const auto aim = [&](int t, mem p, int64_t stride, int64_t step, mem (&x)[LOADS]) __attribute__((always_inline)) {
@@ -670,10 +678,13 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         const uint32_t bits = (uint32_t)(mask >> (32 * sub));
         if (bits != ~0u || c0 + 32 > wave_first) {
             asm volatile("");                                                       // (a branch, not 16 selects in every step)
+            const uint32_t mine = bits >> (4 * half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = 8 * (i >> 2) + 4 * half + (i & 3);
-                s[i] = ((bits >> key) & 1) && c0 + key < lim ? s[i] : NEG_INF;
+            for (int i = 0; i < 16; ++i) s[i] = admit(s[i], spread_bit(mine, 8 * (i >> 2) + (i & 3)));
+            if (c0 + 32 > wave_first) {                                             // (causal calls)
+                asm volatile("");
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = c0 + 8 * (i >> 2) + 4 * half + (i & 3) < lim ? s[i] : NEG_INF;
             }
             top = most(s);
         }
@@ -761,7 +772,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         f32x16 sa, sb;
         mem from[LOADS];
         int now = 0, behind = 1, fetched = 2;                                           // K buffers of tiles t, t + 1, t + 2
-        mask = admitted(t0);
+        mask = admitted(t0, flag_of(t0));
         // this thread's first row of the tile that is loaded next
         mem k_from = kp + (int64_t)t0 * MANY_KEYS * a.k_stride[1], v_from = vp + (int64_t)t0 * MANY_KEYS * a.v_stride[1];
         const int64_t k_tile = MANY_KEYS * a.k_stride[1], v_tile = MANY_KEYS * a.v_stride[1];
@@ -790,7 +801,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         for (int t = t0; t < t1; ++t) {
             // (behind the last tile the last one is loaded again, and scores are taken of what LDS holds: neither is used)
             const int tk = min(t + 2, t1 - 1), tv = min(t + 1, t1 - 1);
-            const uint64_t next_mask = admitted(tv);
+            const uint32_t next_flag = flag_of(tv);
             if (t + 2 < t1) k_from += k_tile;
             if (t + 1 < t1) v_from += v_tile;
             aim(tk, k_from, a.k_stride[1], k_step, from);
@@ -801,8 +812,8 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
             step(t, 1, sb, top, s_k[behind], s_k[behind] + 32 * PITCH, sa, from, vr, s_v[(t + 1) & 1]);
             if (t + 1 < t1) {
                 put_k(fetched);
-                put_v(t + 1, next_mask);
-                mask = next_mask;
+                mask = admitted(t + 1, next_flag);
+                put_v(t + 1, mask);
                 meet();
                 const int free = now;
                 now = behind;
@@ -904,7 +915,7 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
 {
     Plan p{};
     p.rows = (int)(tq * (heads / kv_heads));
-    p.many = sixteen && p.rows > 32;
+    p.many = sixteen && p.rows > 40;            // (48 rows of 64 over 1000 states: 51 us and 55 with the other, 40 rows: 23 and 20)
     if (p.many) {
         p.tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
         const int64_t wgs = n * kv_heads * p.tiles, most = tk / (MANY_KEYS * 8);
