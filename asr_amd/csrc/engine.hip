@@ -3,6 +3,7 @@
 // /root/reference/transformer/.
 #include "asr_common.h"
 #include "../../include/asr_amd.h"
+#include "ops_common.h"
 
 #include <math.h>
 #include <stdio.h>
@@ -12,6 +13,7 @@
 #include <deque>
 #include <map>
 #include <memory>
+#include <new>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1248,6 +1250,19 @@ int with_range_retry(asr_handle* h, F&& run)
 // =================================================================================================
 // C ABI
 // =================================================================================================
+// device buffers of one call, released on return
+struct CallBufs {
+    asr_handle* h;
+    std::vector<void*> p;
+    ~CallBufs() { for (void* q : p) dev_free(h, q); }
+    template <typename T> int get(T** out, size_t count)
+    {
+        int r = dev_alloc_t(h, out, count);
+        if (!r) p.push_back(*out);
+        return r;
+    }
+};
+
 extern "C" {
 
 int asr_device_count(void)
@@ -1644,41 +1659,28 @@ int asr_decode_groups(asr_handle* h, const float* X, int32_t n_groups, const int
     return with_range_retry(h, [&]() { return asr_decode_groups_once(h, X, n_groups, n_g, t_g, d, Y, y_capacity, len_out); });
 }
 
-// Replaces Evaluator.loss (evaluate.py:49-50): sess.run(model.loss_sum) for one tower = encoder, teacher-forced
-// decoder_impl on shift_right(Y) (model.py:171,492-557) and test_loss (model.py:350-360).
-static int asr_loss_once(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, double* loss_sum)
+// Encoder and teacher-forced decoder_impl on shift_right(Y) (model.py:171,492-557): logits [n * ty, V] of every target position, queued on the
+// handle's stream; *dY: the targets on the device
+static int teacher_forced_logits(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, CallBufs& tmp,
+                                 float** logits, int32_t** dY)
 {
-    if (!h || !loss_sum || (n > 0 && (!X || !Y))) return h ? fail(h, ASR_ERR_ARG, "null argument") : ASR_ERR_ARG;
-    *loss_sum = 0.0;
-    if (!h->finalized) return fail(h, ASR_ERR_STATE, "asr_finalize_weights has not succeeded on this handle");
-    int rc = set_device(h);
-    if (rc) return rc;
-    if ((rc = check_xshape(h, n, t, d))) return rc;
-    if (n == 0) return ASR_OK;                                                  // model.py:184-187: loss 0.0
-    if (ty < 1 || ty > 16384) return fail(h, ASR_ERR_ARG, "target length must be in 1..16384");
+    int rc;
     if ((rc = ensure_encoder_capacity(h, n, t))) return rc;
     if ((rc = ensure_pe(h, std::max(t, ty)))) return rc;
     hipStream_t s = h->stream;
     const int H = h->H, F = h->F, M = n * t, Md = n * ty;
     const size_t MH = (size_t)Md * H;
-    struct Tmp {                                                                // per-call workspaces, released on return
-        asr_handle* h; std::vector<void*> p;
-        ~Tmp() { for (void* q : p) dev_free(h, q); }
-    } tmp{h, {}};
-    auto getf = [&](float** out, size_t count) { int r = dev_alloc_t(h, out, count); if (!r) tmp.p.push_back(*out); return r; };
-    int32_t* dY = nullptr;
-    float *y0, *z1, *z2, *ctx, *part, *qkv, *kv, *hid, *logits, *rowl;
-    if ((rc = dev_alloc_t(h, &dY, (size_t)Md))) return rc;
-    tmp.p.push_back(dY);
-    if ((rc = getf(&y0, MH)) || (rc = getf(&z1, MH)) || (rc = getf(&z2, MH)) || (rc = getf(&ctx, MH)) || (rc = getf(&part, MH)) ||
-        (rc = getf(&qkv, 3 * MH)) || (rc = getf(&kv, (size_t)M * 2 * H)) || (rc = getf(&hid, (size_t)Md * F)) ||
-        (rc = getf(&logits, (size_t)Md * h->V)) || (rc = getf(&rowl, (size_t)Md)))
+    float *y0, *z1, *z2, *ctx, *part, *qkv, *kv, *hid;
+    if ((rc = tmp.get(dY, (size_t)Md))) return rc;
+    if ((rc = tmp.get(&y0, MH)) || (rc = tmp.get(&z1, MH)) || (rc = tmp.get(&z2, MH)) || (rc = tmp.get(&ctx, MH)) || (rc = tmp.get(&part, MH)) ||
+        (rc = tmp.get(&qkv, 3 * MH)) || (rc = tmp.get(&kv, (size_t)M * 2 * H)) || (rc = tmp.get(&hid, (size_t)Md * F)) ||
+        (rc = tmp.get(logits, (size_t)Md * h->V)))
         return rc;
     HIP_TRY(h, hipMemcpyAsync(h->xin, X, (size_t)M * d * sizeof(float), hipMemcpyHostToDevice, s));
-    HIP_TRY(h, hipMemcpyAsync(dY, Y, (size_t)Md * sizeof(int32_t), hipMemcpyHostToDevice, s));
+    HIP_TRY(h, hipMemcpyAsync(*dY, Y, (size_t)Md * sizeof(int32_t), hipMemcpyHostToDevice, s));
     if ((rc = run_encoder(h, h->xin, n, t))) return rc;                         // -> h->x0, h->pad2
     const float mult = h->cfg.scale_embedding ? (float)sqrt((double)H) : 1.0f;
-    HIP_TRY(h, launch_embed_shifted(h->emb, dY, Md, ty, h->V, h->pe, mult, H, y0, s));            // model.py:500-508
+    HIP_TRY(h, launch_embed_shifted(h->emb, *dY, Md, ty, h->V, h->pe, mult, H, y0, s));            // model.py:500-508
     for (int l = 0; l < h->L; ++l) {
         const DecBlock& b = h->dec[l];
         if ((rc = gemm(h, y0, b.wqkv, b.bqkv, qkv, Md, 3 * H, H, EPI_BIAS, 1))) return rc;
@@ -1695,7 +1697,28 @@ static int asr_loss_once(asr_handle* h, const float* X, int32_t n, int32_t t, in
         HIP_TRY(h, launch_add_layer_norm(z2, part, 1, 0, b.b2, b.ln2s, b.ln2b, nullptr, nullptr, Md, H, y0, s));        // :547-555
     }
     const float* wout = h->cfg.tie_embedding_and_softmax ? h->emb_gemm : h->softmax_w;
-    if ((rc = gemm(h, y0, wout, nullptr, logits, Md, h->V, H, EPI_BIAS, 1))) return rc;            // :353-355
+    if ((rc = gemm(h, y0, wout, nullptr, *logits, Md, h->V, H, EPI_BIAS, 1))) return rc;            // :353-355
+    return ASR_OK;
+}
+
+// Replaces Evaluator.loss (evaluate.py:49-50): sess.run(model.loss_sum) for one tower = the teacher-forced logits and test_loss (model.py:350-360).
+static int asr_loss_once(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, double* loss_sum)
+{
+    if (!h || !loss_sum || (n > 0 && (!X || !Y))) return h ? fail(h, ASR_ERR_ARG, "null argument") : ASR_ERR_ARG;
+    *loss_sum = 0.0;
+    if (!h->finalized) return fail(h, ASR_ERR_STATE, "asr_finalize_weights has not succeeded on this handle");
+    int rc = set_device(h);
+    if (rc) return rc;
+    if ((rc = check_xshape(h, n, t, d))) return rc;
+    if (n == 0) return ASR_OK;                                                  // model.py:184-187: loss 0.0
+    if (ty < 1 || ty > 16384) return fail(h, ASR_ERR_ARG, "target length must be in 1..16384");
+    CallBufs tmp{h, {}};
+    float *logits = nullptr, *rowl = nullptr;
+    int32_t* dY = nullptr;
+    if ((rc = teacher_forced_logits(h, X, n, t, d, Y, ty, tmp, &logits, &dY))) return rc;
+    const int Md = n * ty;
+    if ((rc = tmp.get(&rowl, (size_t)Md))) return rc;
+    hipStream_t s = h->stream;
     HIP_TRY(h, launch_xent_rows(logits, dY, Md, h->V, rowl, s));
     std::vector<float> rl((size_t)Md);
     HIP_TRY(h, hipMemcpyAsync(rl.data(), rowl, rl.size() * sizeof(float), hipMemcpyDeviceToHost, s));
@@ -1710,6 +1733,55 @@ int asr_loss(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, con
 {
     if (!h) return ASR_ERR_ARG;
     return with_range_retry(h, [&]() { return asr_loss_once(h, X, n, t, d, Y, ty, loss_sum); });
+}
+
+// Token by token: the teacher-forced logits and token_logprobs (ops_rows.hip) on them.
+static int asr_score_once(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, int32_t top, float* logprob,
+                          float* entropy, float* top_logprobs, int32_t* top_tokens)
+{
+    if (n > 0 && (!X || !Y || !logprob || !entropy || (top > 0 && (!top_logprobs || !top_tokens)))) return fail(h, ASR_ERR_ARG, "null argument");
+    if (!h->finalized) return fail(h, ASR_ERR_STATE, "asr_finalize_weights has not succeeded on this handle");
+    int rc = set_device(h);
+    if (rc) return rc;
+    if ((rc = check_xshape(h, n, t, d))) return rc;
+    if (top < 0 || top > 32 || top > h->V) return fail(h, ASR_ERR_ARG, "top must be in 0..min(32, dst_vocab_size)");
+    if (n == 0) return ASR_OK;
+    if (ty < 1 || ty > 16384) return fail(h, ASR_ERR_ARG, "target length must be in 1..16384");
+    const size_t Md = (size_t)n * ty;
+    std::vector<int32_t> tokens(Y, Y + Md);                                     // (outlives the device buffers, whose release waits for the copies)
+    CallBufs tmp{h, {}};
+    for (int32_t& v : tokens)
+        if (v == 0) v = -1;                                                     // padding: "no token"
+    float *logits = nullptr, *dlp, *dh, *dtl = nullptr;
+    int32_t *dY = nullptr, *dtok, *dtt = nullptr;
+    if ((rc = teacher_forced_logits(h, X, n, t, d, Y, ty, tmp, &logits, &dY))) return rc;
+    if ((rc = tmp.get(&dtok, Md)) || (rc = tmp.get(&dlp, Md)) || (rc = tmp.get(&dh, Md))) return rc;
+    if (top > 0 && ((rc = tmp.get(&dtl, Md * top)) || (rc = tmp.get(&dtt, Md * top)))) return rc;
+    hipStream_t s = h->stream;
+    HIP_TRY(h, hipMemcpyAsync(dtok, tokens.data(), Md * sizeof(int32_t), hipMemcpyHostToDevice, s));
+    asr_token_logprobs_args a{};
+    a.logits = logits; a.tokens = dtok; a.logprob = dlp; a.entropy = dh; a.top_logprobs = dtl; a.top_tokens = dtt;
+    a.rows = (int64_t)Md; a.row_stride = h->V; a.vocab = h->V; a.top = top; a.dtype = ASR_F32; a.token_bytes = 4;
+    if ((rc = ops_token_logprobs(a, s))) return fail(h, rc, asr_ops_last_error());
+    HIP_TRY(h, hipMemcpyAsync(logprob, dlp, Md * sizeof(float), hipMemcpyDeviceToHost, s));
+    HIP_TRY(h, hipMemcpyAsync(entropy, dh, Md * sizeof(float), hipMemcpyDeviceToHost, s));
+    if (top > 0) {
+        HIP_TRY(h, hipMemcpyAsync(top_logprobs, dtl, Md * top * sizeof(float), hipMemcpyDeviceToHost, s));
+        HIP_TRY(h, hipMemcpyAsync(top_tokens, dtt, Md * top * sizeof(int32_t), hipMemcpyDeviceToHost, s));
+    }
+    HIP_TRY(h, hipStreamSynchronize(s));
+    return ASR_OK;
+}
+
+int asr_score(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, int32_t top, float* logprob, float* entropy,
+              float* top_logprobs, int32_t* top_tokens)
+{
+    if (!h) return ASR_ERR_ARG;
+    try {
+        return with_range_retry(h, [&]() { return asr_score_once(h, X, n, t, d, Y, ty, top, logprob, entropy, top_logprobs, top_tokens); });
+    } catch (const std::bad_alloc&) {
+        return fail(h, ASR_ERR_CAPACITY, "out of memory");
+    }
 }
 
 int asr_stack_frames(asr_handle* h, const float* feats, int32_t n_frames, int32_t dim, int32_t left, int32_t right, int32_t sub,

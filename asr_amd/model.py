@@ -170,6 +170,22 @@ class Engine(object):
         _lib.check(self._h, lib.asr_loss(self._h, _lib.fptr(X), n, t, d, _lib.iptr(Y), Y.shape[1], C.byref(out)))
         return float(out.value)
 
+    def score(self, X, Y, top=0):
+        """Token by token what `loss` adds up: X float32 [n, t, d], Y int32 [n, ty] (0 = padding) -> (logprob [n, ty], entropy [n, ty],
+        top_logprobs [n, ty, top], top_tokens [n, ty, top]): log p of every target given the ones before it (0 for padding), the
+        entropy of its distribution and the `top` (at most 32) most likely tokens there (`asr_score`)."""
+        X = _lib.f32(X)
+        Y = _lib.i32(Y)
+        if X.ndim != 3 or Y.ndim != 2 or Y.shape[0] != X.shape[0]:
+            raise ValueError('Y must be [n, ty] with the batch size of X')
+        n, t, d = X.shape
+        ty, top = Y.shape[1], int(top)
+        logprob, entropy = np.zeros((n, ty), np.float32), np.zeros((n, ty), np.float32)
+        top_logprobs, top_tokens = np.zeros((n, ty, max(top, 0)), np.float32), np.zeros((n, ty, max(top, 0)), np.int32)
+        _lib.check(self._h, lib.asr_score(self._h, _lib.fptr(X), n, t, d, _lib.iptr(Y), ty, top, _lib.fptr(logprob), _lib.fptr(entropy),
+                                          _lib.fptr(top_logprobs), _lib.iptr(top_tokens)))
+        return logprob, entropy, top_logprobs, top_tokens
+
     def decode_dev(self, ptr, n, t, d, raw=None):
         """Device-resident input (bench): `ptr` = device address of X [n,t,d], or with
         raw=(raw_frames, raw_dim, left, right, sub) of RAW fbank [n, raw_frames, raw_dim]."""
@@ -641,6 +657,16 @@ class Model(object):
             if b > a:
                 total += self.engines[i % len(self.engines)].loss(X[a:b], Y[a:b])
         return total
+
+    def score(self, X, Y, top=0):
+        """Engine.score over the towers' shards (the split of `loss`), rows in the order of X."""
+        X = np.asarray(X, dtype=np.float32)
+        Y = np.asarray(Y, dtype=np.int32)
+        parts = [self.engines[i % len(self.engines)].score(X[a:b], Y[a:b], top)
+                 for i, (a, b) in enumerate(shard_bounds(X.shape[0], self._num_towers)) if b > a]
+        if not parts:
+            return self.engines[0].score(X, Y, top)
+        return tuple(np.concatenate(p, axis=0) for p in zip(*parts))
 
 
 class Transformer(Model):

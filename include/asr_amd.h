@@ -151,6 +151,14 @@ int asr_decode_dev(asr_handle* h, const float* X_dev, int32_t n, int32_t t, int3
 int asr_loss(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d,
              const int32_t* Y, int32_t ty, double* loss_sum);
 
+/* What asr_loss adds up, token by token, and how sure the model was: the same teacher-forced pass over Y int32 [n, ty] (0 = padding), then for
+ * every position logprob [n, ty] = log p(Y | the targets before it, X), entropy [n, ty] of that distribution, and top_tokens / top_logprobs [n, ty, top] =
+ * its `top` (0 .. 32) most likely tokens, ties to the lower one (asr_token_logprobs below).  Padding has log probability 0, and the distribution's
+ * entropy and alternatives like every position.  Confidence of hypotheses and rescoring of n-best lists need these; the reference only
+ * has the sum (model.py:350-360: loss_sum = minus the sum of logprob over Y != 0). */
+int asr_score(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, int32_t top, float* logprob,
+              float* entropy, float* top_logprobs, int32_t* top_tokens);
+
 /* Front end alone.  Replaces tf_fea_splice (+ the `sub` subsampling implied by the
  * `feats.scp.left3_sub3` inputs): feats [n_frames, dim] -> out [ceil(n_frames/sub), dim*(left+right+1)]. */
 int asr_stack_frames(asr_handle* h, const float* feats, int32_t n_frames, int32_t dim,
