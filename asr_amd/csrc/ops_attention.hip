@@ -499,7 +499,7 @@ __device__ inline u32x2 lds_read_transposed(const char* p)
 __device__ inline void load_to_lds(mem p, char* lds)
 {
     const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory", "m0");
 }
 __device__ inline void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ inline float halves_max(float x)

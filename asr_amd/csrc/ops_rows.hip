@@ -514,8 +514,11 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream)
         return ops_fail(ASR_ERR_ARG, "kv8_append: rows of k and v must start on 16 bytes");
     if (((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) || a->cache_stride[0] % 16 || a->cache_stride[1] % 16)
         return ops_fail(ASR_ERR_ARG, "kv8_append: cache rows must start on 16 bytes");
-    if (a->n > 65535 || a->kv_heads > (1 << 20) || (int64_t)a->new_tokens > 65000 * (int64_t)ASR_KV8_BLOCK)
-        return ops_fail(ASR_ERR_ARG, "kv8_append: at most 65535 sequences, 2^20 heads and 65000 blocks of tokens a call");
+    // blocks that new_tokens tokens can touch, wherever the first one falls
+    const int64_t touched = ((int64_t)a->new_tokens + ASR_KV8_BLOCK - 2) / ASR_KV8_BLOCK + 1;
+    const int64_t blocks = touched < a->capacity / ASR_KV8_BLOCK ? touched : a->capacity / ASR_KV8_BLOCK;
+    if (a->n > 65535 || a->kv_heads > (1 << 20) || blocks > 65535)
+        return ops_fail(ASR_ERR_ARG, "kv8_append: at most 65535 sequences, 2^20 heads and 65535 blocks of tokens a call");
     Kv8AppendArgs k{};
     k.x[0] = a->k; k.x[1] = a->v;
     k.cache[0] = a->k_cache; k.cache[1] = a->v_cache;
@@ -524,10 +527,7 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream)
     for (int i = 0; i < 3; ++i) { k.stride[0][i] = a->k_stride[i]; k.stride[1][i] = a->v_stride[i]; }
     k.cache_stride[0] = a->cache_stride[0]; k.cache_stride[1] = a->cache_stride[1];
     k.new_tokens = a->new_tokens; k.kv_heads = a->kv_heads; k.d = a->d; k.capacity = a->capacity;
-    // blocks that new_tokens tokens can touch, wherever the first one falls
-    const int64_t touched = ((int64_t)a->new_tokens + ASR_KV8_BLOCK - 2) / ASR_KV8_BLOCK + 1;
-    const int blocks = (int)(touched < a->capacity / ASR_KV8_BLOCK ? touched : a->capacity / ASR_KV8_BLOCK);
-    const dim3 grid(2 * a->kv_heads, blocks, a->n);
+    const dim3 grid(2 * a->kv_heads, (uint32_t)blocks, a->n);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return ops_launched("kv8_append", a->dtype == ASR_F32 ? run_kv8_append<ASR_F32>(k, grid, s)
                                       : a->dtype == ASR_BF16 ? run_kv8_append<ASR_BF16>(k, grid, s) : run_kv8_append<ASR_F16>(k, grid, s));

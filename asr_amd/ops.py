@@ -47,40 +47,46 @@ def _call(fn, packed, device):
 
 
 # The checks below run before every call: a message is only put together when it is needed.
+def _refused(name, *tensors):
+    """Why these tensors (None entries are skipped) cannot be used together: they are not all on one GPU, or want gradients."""
+    device = tensors[0].get_device()
+    if device < 0:
+        return ValueError('%s: tensors must be in GPU memory' % name)
+    if any(t is not None and t.get_device() != device for t in tensors):
+        return ValueError('%s: all tensors must be on one device' % name)
+    return ValueError('%s has no backward pass: detach its inputs or call it under torch.no_grad()' % name)
+
+
 def _device(name, *tensors):
     """The number of the one device that holds all tensors (None entries are skipped)."""
     device = tensors[0].get_device()
-    if device < 0:
-        raise ValueError('%s: tensors must be in GPU memory' % name)
     grads = torch.is_grad_enabled()
     for t in tensors:
-        if t is None:
-            continue
-        if t.get_device() != device:
-            raise ValueError('%s: all tensors must be on one device' % name)
-        if grads and t.requires_grad:
-            raise ValueError('%s has no backward pass: detach its inputs or call it under torch.no_grad()' % name)
+        if t is not None and (t.get_device() != device or (grads and t.requires_grad)):
+            raise _refused(name, *tensors)
+    if device < 0:
+        raise _refused(name, *tensors)
     return device
 
 
 def _counts(name, what, t, n):
-    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise ValueError('%s: %s must be int32 [%d], contiguous' % (name, what, n))
 
 
-def _rows(name, what, t, n, rows, heads, d):
-    """Strides of a [n, rows, heads, d] tensor whose last dimension is contiguous."""
-    if t.shape != (n, rows, heads, d):
-        raise ValueError('%s: %s must be %s, not %s' % (name, what, [n, rows, heads, d], list(t.shape)))
-    s = t.stride()
-    if s[3] != 1 and d != 1:
+def _rows(name, what, t, dims):
+    """Strides of a tensor of these dimensions [n, rows, heads, d] whose last one is contiguous."""
+    if t.shape != dims:
+        raise ValueError('%s: %s must be %s, not %s' % (name, what, list(dims), list(t.shape)))
+    a, b, c, one = t.stride()
+    if one != 1 and dims[3] != 1:
         raise ValueError('%s: the last dimension of %s must be contiguous' % (name, what))
-    return s[:3]
+    return a, b, c
 
 
 def _output(name, q, out):
     if out is None:
-        return q.new_empty(q.shape)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.dtype != q.dtype or out.shape != q.shape:
         raise ValueError('%s: out must have the shape and type of q' % name)
     if not all(s > 0 or n <= 1 for s, n in zip(out.stride(), out.shape)):
@@ -147,15 +153,16 @@ def cross_attention(q, k, v, lens=None, pad=None, scale=None, out=None):
     name = 'cross_attention'
     device = _device(name, q, k, v, lens, pad, out)
     dtype = _DTYPES.get(q.dtype)
-    if dtype is None or k.dtype != q.dtype or v.dtype != q.dtype:
+    if dtype is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError('%s: q, k and v must be float32, bfloat16 or float16, all the same' % name)
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError('%s: q must be [n, tq, heads, d] and k [n, tk, kv_heads, d]' % name)
-    n, tq, heads, d = q.shape
+    n, tq, heads, d = dims = q.shape
     _, tk, kv_heads, _ = k.shape
-    qs = _rows(name, 'q', q, n, tq, heads, d)
-    ks = _rows(name, 'k', k, n, tk, kv_heads, d)
-    vs = _rows(name, 'v', v, n, tk, kv_heads, d)
+    kv_dims = (n, tk, kv_heads, d)
+    qs = _rows(name, 'q', q, dims)
+    ks = _rows(name, 'k', k, kv_dims)
+    vs = _rows(name, 'v', v, kv_dims)
     if lens is not None:
         _counts(name, 'lens', lens, n)
     pad_stride = 0
@@ -209,13 +216,14 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, lens, counts=None):
     device = _device(name, k, v, k_cache, v_cache, k_scale, v_scale, lens, counts)
     n, kv_heads, capacity, d, cs = _cache(name, k_cache, v_cache, k_scale, v_scale)
     dtype = _DTYPES.get(k.dtype)
-    if dtype is None or v.dtype != k.dtype:
+    if dtype is None or v.dtype is not k.dtype:
         raise ValueError('%s: k and v must be float32, bfloat16 or float16, both the same' % name)
     if k.dim() != 4:
         raise ValueError('%s: k must be [n, new, kv_heads, d]' % name)
     new = k.shape[1]
-    ks = _rows(name, 'k', k, n, new, kv_heads, d)
-    vs = _rows(name, 'v', v, n, new, kv_heads, d)
+    dims = (n, new, kv_heads, d)
+    ks = _rows(name, 'k', k, dims)
+    vs = _rows(name, 'v', v, dims)
     if (cs[0] <= 0 and n > 1) or (cs[1] <= 0 and kv_heads > 1):
         raise ValueError('%s: the caches must not be expanded' % name)
     _counts(name, 'lens', lens, n)
@@ -241,7 +249,7 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, sca
     if q.dim() != 4:
         raise ValueError('%s: q must be [n, tq, heads, d]' % name)
     _, tq, heads, _ = q.shape
-    qs = _rows(name, 'q', q, n, tq, heads, d)
+    qs = _rows(name, 'q', q, (n, tq, heads, d))
     _counts(name, 'lens', lens, n)
     out = _output(name, q, out)
     size = _kv8_workspace(n, tq, capacity, heads, kv_heads, d, dtype)
