@@ -84,6 +84,13 @@ template <bool HI> __device__ inline uint32_t codes_bf16(uint32_t w, float scale
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, HI));
 }
 
+// all ones in the bytes of w that are NaN codes (all seven bits below the sign set)
+__device__ inline uint32_t nan_codes(uint32_t w)
+{
+    const uint32_t top = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return top | (top - (top >> 7));
+}
+
 // all ones where bit `at` of `bits` is set; x there, else -infinity (two instructions a value)
 __device__ inline uint32_t spread_bit(uint32_t bits, int at) { return (uint32_t)((int32_t)(bits << (31 - at)) >> 31); }
 __device__ inline float admit(float x, uint32_t ones) { return __uint_as_float((__float_as_uint(x) & ones) | (0xff800000u & ~ones)); }
@@ -138,7 +145,7 @@ __device__ inline int place_of(int nbh, int per, int64_t& id)
 // P as PTERMS (two: 2^-17 / 2^-22 of it lost, three: nothing), which costs matrix instructions that a loop waiting for memory has to spare.
 // float32 K / V are cut into three bf16 terms as well (8 + 8 + 8 bits: exact), and of the nine products the six above 2^-24 are taken: the 16-bit matrix
 // pipe is 16 times the float32 one, which besides shares its units with the vector instructions (50 x 61 queries over 1000 states of 16 heads:
-// 133 us on the float32 instruction).
+// 133 us on the float32 instruction, 108 so).
 template <int QT, int KVT, int DP, int NQ> struct Few {
     static constexpr bool MATH32 = KVT == KV_F32, F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
     static constexpr int QTERMS = QT == ASR_F32 ? 3 : CODES && QT == ASR_F16 ? 2 : 1;
@@ -311,6 +318,7 @@ void attention_few_kernel(AttnArgs a)
         }
     };
 
+    uint64_t nan_seen = 0;
     int chunk = chunk0 + wave;
     if (chunk < chunk1) {
         load_k(32 * chunk);
@@ -386,6 +394,21 @@ void attention_few_kernel(AttnArgs a)
 #pragma unroll
             for (int j = 0; j < 8; ++j) vr[j] &= spread_bit(mine, j);
         }
+        // What a causal call hides from some of the rows may be NaN as well: such values are taken as 0 and looked up again at the end
+        if constexpr (F::CODES) {
+            if (c0 + 32 > first_lim) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int w = 0; w < F::VW; ++w) {
+                        const uint32_t x = nan_codes(vr[j][w]);
+                        any |= x;
+                        vr[j][w] &= ~x;
+                    }
+                nan_seen |= __ballot(any != 0);
+            }
+        }
         u32x4 pf[NQ][F::PTERMS];
 #pragma unroll
         for (int t = 0; t < NQ; ++t)
@@ -420,6 +443,25 @@ void attention_few_kernel(AttnArgs a)
             for (int t = 0; t < NQ; ++t) o[t][i] = mfma_terms<F::F16>(vf, pf[t], o[t][i]);
         }
         if (more) load_v(c0 + 32 * FEW_WAVES);
+    }
+
+    if constexpr (F::CODES) {
+        if (nan_seen) {
+            // where a row sees a NaN its sum is one (this wave's chunks; a lane has DP / 16 columns from DP / 16 (4 g + j) on)
+            for (int c = chunk0 + wave; c < chunk1; c += FEW_WAVES)
+                for (int key = 32 * c; 32 * c + 32 > first_lim && key < min(32 * c + 32, len); ++key)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int w = 0; w < F::VW; ++w) {
+                            const int at = DP / 16 * (4 * g + j) + 4 * w;
+                            const uint32_t x = at < a.d ? nan_codes(load_as<uint32_t>((mem)vb + (int64_t)key * a.v_stride[1] + at)) : 0u;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                for (int t = 0; t < NQ; ++t) o[t][4 * w + e][j] = key < lim[t] && (x >> (8 * e)) & 1 ? __builtin_nanf("") : o[t][4 * w + e][j];
+                        }
+        }
     }
 
     // join the waves
@@ -541,6 +583,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     const int len = keys_of(a, b), row0 = tile * MANY_ROWS;
     int last_key = len;
     if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + MANY_ROWS - 1, a.rows - 1) / a.group + 1));
+    const int first_lim = a.causal ? len - a.tq + row0 / a.group + 1 : 0x7fffffff;       // every row of this workgroup sees the keys below it
     const int all_tiles = (last_key + MANY_KEYS - 1) / MANY_KEYS, share = (all_tiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * share, t1 = min(all_tiles, t0 + share);
 
@@ -623,7 +666,9 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     const auto put_k = [&](int buf) __attribute__((always_inline)) {
         if constexpr (!DIRECT) put(kr, s_k[buf], ks, turn_k);
     };
-    // what is not admitted may hold anything: V = 0 meets P = 0
+    // what is not admitted may hold anything: V = 0 meets P = 0.  What a causal call hides from some of the rows may be NaN as well: such values
+    // are taken as 0 and looked up again at the end.
+    uint64_t nan_seen = 0;
     const auto put_v = [&](int t, uint64_t mask) __attribute__((always_inline)) {
         if constexpr (DIRECT) {
             if (mask == ~0ull) return;
@@ -636,6 +681,20 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
 #pragma unroll
                 for (int u = 0; u < LOADS; ++u)
                     if (!((mask >> (my_row + u * LOAD_ROWS)) & 1)) vr[u] = u32x4{};
+            }
+            if constexpr (CODES) {
+                if ((t + 1) * MANY_KEYS > first_lim) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int u = 0; u < LOADS; ++u)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t x = in ? nan_codes(vr[u][w]) : 0u;
+                            any |= x;
+                            vr[u][w] &= ~x;
+                        }
+                    nan_seen |= __ballot(any != 0);
+                }
             }
             put(vr, s_v[t & 1], vs, turn_v);
         }
@@ -822,6 +881,28 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
             }
         }
         wait_for_memory();                                                              // (no load into LDS may outlive its workgroup)
+        if constexpr (CODES) {
+            if (a.causal) {
+                uint32_t* waves = reinterpret_cast<uint32_t*>(s_k);                     // (LDS is full: two workgroups share it)
+                __syncthreads();
+                if (lane == 0) waves[wave] = nan_seen != 0;
+                __syncthreads();
+                if (waves[0] | waves[1] | waves[2] | waves[3]) {
+                    // where this lane's row sees a NaN its sum is one
+                    const int to = min(t1 * MANY_KEYS, lim);
+                    for (int key = max(t0, first_lim >> 6) * MANY_KEYS; key < to; ++key)
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int at = 32 * i + 8 * j + 4 * half;
+                                const uint32_t x = at < a.d ? nan_codes(load_as<uint32_t>((mem)vb + (int64_t)key * a.v_stride[1] + at)) : 0u;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[i][4 * j + e] = (x >> (8 * e)) & 1 ? __builtin_nanf("") : o[i][4 * j + e];
+                            }
+                }
+            }
+        }
     }
 
     if (r >= a.rows) return;

@@ -412,9 +412,11 @@ template <int DT, int NT, int ITEMS> __global__ __launch_bounds__(NT) void kv8_a
     if (held < 0 || held >= a.capacity) return;
     const int count = a.counts ? min(a.counts[b], a.new_tokens) : a.new_tokens;
     const int end = (int)min((int64_t)a.capacity, (int64_t)held + count);        // positions held .. end get tokens
-    const int block = held / ASR_KV8_BLOCK + blockIdx.y, first = block * ASR_KV8_BLOCK;
+    const int block = held / ASR_KV8_BLOCK + blockIdx.y;
+    if (block >= a.capacity / ASR_KV8_BLOCK) return;
+    const int first = block * ASR_KV8_BLOCK;
     const int lo = max(held, first), hi = min(end, first + ASR_KV8_BLOCK);
-    if (block >= a.capacity / ASR_KV8_BLOCK || lo >= hi) return;
+    if (lo >= hi) return;
     const int tid = threadIdx.x, per_row = a.d / PER, items = (hi - lo) * per_row;
     const T* x = static_cast<const T*>(a.x[which]) + (int64_t)b * a.stride[which][0] + (int64_t)h * a.stride[which][2] + (int64_t)(lo - held) * a.stride[which][1];
     uint8_t* codes = a.cache[which] + (int64_t)b * a.cache_stride[0] + (int64_t)h * a.cache_stride[1] + (int64_t)first * a.d;
@@ -484,7 +486,7 @@ template <int DT> hipError_t run_kv8_append(const Kv8AppendArgs& k, dim3 grid, h
 {
     constexpr int PER = Elem<DT>::PER;
     // a few tokens: one wave holds a block's share (64 sequences, one token, 16 heads: 4.7 us with four waves)
-    if (k.new_tokens * k.d <= 64 * PER) return ops_launch(kv8_append_kernel<DT, 64, 1>, grid, dim3(64), s, k);
+    if ((int64_t)k.new_tokens * k.d <= 64 * PER) return ops_launch(kv8_append_kernel<DT, 64, 1>, grid, dim3(64), s, k);
     if (k.d <= 64) return ops_launch(kv8_append_kernel<DT, 256, 64 * 64 / PER / 256>, grid, dim3(256), s, k);
     return ops_launch(kv8_append_kernel<DT, 256, 64 * 128 / PER / 256>, grid, dim3(256), s, k);
 }
@@ -519,6 +521,7 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream)
     const int64_t blocks = touched < a->capacity / ASR_KV8_BLOCK ? touched : a->capacity / ASR_KV8_BLOCK;
     if (a->n > 65535 || a->kv_heads > (1 << 20) || blocks > 65535)
         return ops_fail(ASR_ERR_ARG, "kv8_append: at most 65535 sequences, 2^20 heads and 65535 blocks of tokens a call");
+    if (a->k_cache == a->v_cache || a->k_scale == a->v_scale) return ops_fail(ASR_ERR_ARG, "kv8_append: keys and values need caches and scales of their own");
     Kv8AppendArgs k{};
     k.x[0] = a->k; k.x[1] = a->v;
     k.cache[0] = a->k_cache; k.cache[1] = a->v_cache;

@@ -113,6 +113,8 @@ def token_logprobs(logits, tokens, top=0):
         raise ValueError('token_logprobs: tokens must have the shape of logits without its last dimension')
     if tokens.dtype is not torch.int32 and tokens.dtype is not torch.int64:
         raise ValueError('token_logprobs: tokens must be int32 or int64')
+    if vocab > 1 << 30:
+        raise ValueError('token_logprobs: a vocabulary of at most 2^30 tokens')
     if not 0 <= top <= min(32, vocab):
         raise ValueError('token_logprobs: top must be in 0..min(32, vocab)')
     if vocab > 1 and logits.stride(-1) != 1:
@@ -133,13 +135,20 @@ def token_logprobs(logits, tokens, top=0):
     return logprob, entropy, top_logprobs, top_tokens
 
 
+def _sizes(name, *sizes):
+    if max(sizes) >= 1 << 31:
+        raise ValueError('%s: sizes must be below 2^31' % name)
+
+
 @functools.lru_cache(maxsize=4096)
 def _cross_workspace(n, tq, tk, heads, kv_heads, d, dtype):
+    _sizes('cross_attention', n, tq, tk, heads)
     return lib.asr_cross_attention_workspace(n, tq, tk, heads, kv_heads, d, dtype)
 
 
 @functools.lru_cache(maxsize=4096)
 def _kv8_workspace(n, tq, capacity, heads, kv_heads, d, dtype):
+    _sizes('kv8_attention', n, tq, capacity, heads)
     return lib.asr_kv8_attention_workspace(n, tq, capacity, heads, kv_heads, d, dtype)
 
 
@@ -176,7 +185,7 @@ def cross_attention(q, k, v, lens=None, pad=None, scale=None, out=None):
     _call(lib.asr_cross_attention,
           _CROSS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lens is None else lens.data_ptr(),
                       0 if pad is None else pad.data_ptr(), 0 if ws is None else ws.data_ptr(), *qs, *ks, *vs, *out.stride()[:3],
-                      pad_stride, size, n, tq, tk, heads, kv_heads, d, dtype, d ** -0.5 if scale is None else scale), device)
+                      pad_stride, size, n, tq, tk, heads, kv_heads, d, dtype, (d or 1) ** -0.5 if scale is None else scale), device)
     return out
 
 
@@ -221,6 +230,8 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, lens, counts=None):
     if k.dim() != 4:
         raise ValueError('%s: k must be [n, new, kv_heads, d]' % name)
     new = k.shape[1]
+    if new >= 1 << 31 or capacity >= 1 << 31:
+        raise ValueError('%s: sizes must be below 2^31' % name)
     dims = (n, new, kv_heads, d)
     ks = _rows(name, 'k', k, dims)
     vs = _rows(name, 'v', v, dims)
@@ -238,7 +249,7 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, lens, counts=None):
 def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, scale=None, out=None):
     """q [n, tq, heads, d] (float32, bfloat16 or float16) over the first lens[b] (int32 [n]) tokens of each sequence's cache ->
     [n, tq, heads, d] of q's type.  causal: query i is the sequence's token lens[b] - tq + i, which the cache already holds, and sees nothing behind
-    itself.  A query with nothing to see gives zeros; what stands behind lens[b] does not matter.  Query head h reads key head
+    itself.  A query with nothing to see gives zeros; what it does not see does not matter, NaN included.  Query head h reads key head
     h // (heads // kv_heads); scale defaults to 1 / sqrt(d); d is a multiple of 16 up to 128."""
     name = 'kv8_attention'
     device = _device(name, q, k_cache, v_cache, k_scale, v_scale, lens, out)
@@ -257,5 +268,5 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, sca
     _call(lib.asr_kv8_attention,
           _ATTEND.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                        lens.data_ptr(), 0 if ws is None else ws.data_ptr(), *qs, *out.stride()[:3], cs[0], cs[1], size, n, tq, heads, kv_heads,
-                       d, capacity, dtype, 1 if causal else 0, d ** -0.5 if scale is None else scale), device)
+                       d, capacity, dtype, 1 if causal else 0, (d or 1) ** -0.5 if scale is None else scale), device)
     return out

@@ -317,9 +317,10 @@ int asr_token_logprobs(const asr_token_logprobs_args* a, void* stream);
  * admitted: j < lens[b] (lens null: all tk; values are taken as 0 below 0 and as tk above tk) and pad[b, j] == 0 (pad null: no flags).  What
  * stands in positions that are not admitted does not matter, NaN and infinity included; a query without an admitted position gives 0.  Beams
  * of one utterance are query rows (tq = beams): nothing orders the queries.
- * q, out: [n, tq, heads, d], k, v: [n, tk, kv_heads, d] of one type (bf16 and f16 are multiplied on the 16-bit matrix instruction, f32 on the
- * exact float32 one; scores, soft-max statistics and sums are float32), d contiguous, every other stride free but such that each row starts on
- * 16 bytes; out may not overlap the inputs.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
+ * q, out: [n, tq, heads, d], k, v: [n, tk, kv_heads, d] of one type, d contiguous, every other stride free but such that each row starts on
+ * 16 bytes; out may not overlap the inputs.  bf16 and f16 are multiplied as they are; f32 is cut into three bf16 terms (exact) of whose nine products the six
+ * above 2^-24 are taken, so an infinity in an admitted f32 position gives NaN; scores, soft-max statistics and sums are float32.  With bf16 and f16 and more
+ * than 40 rows (tq * heads / kv_heads) the probabilities are rounded once to that type.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
 typedef struct asr_cross_attention_args {
     const void *q, *k, *v;
     void* out;
@@ -346,7 +347,7 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream);
  * every finite magnitude it was made for stays within 448, the largest e4m3 value; a value is rounded once, to the nearest code, halves to
  * even.  A block that held tokens before (lens[b] inside it) keeps its scale or takes the larger one its new tokens need; its older tokens are then
  * coded again under it.  Infinities are held as +-448, NaN stays NaN; neither counts for a scale.  Nothing else is written: blocks
- * without new tokens, and positions behind the last one, stay as they are.  No two sequences may share cache memory.
+ * without new tokens, and positions behind the last one, stay as they are.  No two sequences may share cache memory, nor may K and V.
  * k, v: [n, new_tokens, kv_heads, d], any asr_dtype, rows on 16 bytes.  d % 16 == 0, 16 <= d <= 128; capacity % ASR_KV8_BLOCK == 0. */
 typedef struct asr_kv8_append_args {
     const void *k, *v;
@@ -363,7 +364,7 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream);
 
 /* asr_cross_attention with the cache above for keys and values; lens[b] tokens are valid (taken as 0 below 0, as the capacity above it).
  * causal: query i of sequence b is its token lens[b] - tq + i and sees nothing behind itself (the cache already holds the tq newest tokens; a
- * query with nothing to see gives 0).  Codes are multiplied exactly on the 16-bit matrix instruction; a q of f16 or f32 enters as
+ * query with nothing to see gives 0; NaN in later tokens does not reach it).  Codes are multiplied exactly on the 16-bit matrix instruction; a q of f16 or f32 enters as
  * two or three bf16 terms, so nothing of it is lost. */
 typedef struct asr_kv8_attention_args {
     const void* q;

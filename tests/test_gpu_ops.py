@@ -377,6 +377,21 @@ def test_kv8_append_extremes(ops):
         _check_append(ops, k.cuda(), -k.cuda(), cache, torch.full((n,), lens, dtype=torch.int32).cuda())
 
 
+def test_kv8_append_of_more_new_tokens_than_fit(ops):
+    """2^25 new tokens of 128 (their product passes 32 bits), the same memory for each, into a cache of 128: what fits is written."""
+    g = _gen(77)
+    cache = _random_cache(ops, g, 1, 1, 128, 128)
+    row = torch.randn(1, 1, 1, 128, generator=g).to(torch.bfloat16).cuda()
+    lens = torch.tensor([3], dtype=torch.int32).cuda()
+    other = [c.clone() for c in cache]
+    many = row.expand(1, 1 << 25, 1, 128)
+    ops.kv8_append(many, many, *cache, lens)
+    few = row.expand(1, 125, 1, 128)
+    ops.kv8_append(few, few, *other, lens)
+    for a, b in zip(cache, other):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_kv8_append_strides_and_views(ops):
     """Keys and values as halves of one projection, caches as part of larger ones: nothing beside them is written."""
     g = _gen(3)
@@ -448,6 +463,38 @@ def test_kv8_attention_lengths(ops, tq, heads, kv_heads, d, causal, dtype):
             s[b, :, (length + 63) // 64:] = math.inf
     q = torch.randn(n, tq, heads, d, generator=g).to(TYPES[dtype]).cuda()
     _check_kv8(ops, q, cache, lens.cuda(), causal=causal, scale=0.2)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('tq,heads,kv_heads,capacity,d', [(1, 2, 2, 128, 64), (9, 4, 2, 192, 128), (24, 2, 1, 128, 80), (8, 2, 2, 2048, 64), (90, 2, 2, 192, 128),
+                                                          (150, 4, 2, 320, 64), (70, 2, 1, 128, 48), (200, 1, 1, 2048, 128)])
+def test_kv8_attention_nan_in_later_tokens(ops, tq, heads, kv_heads, capacity, d, dtype):
+    """A causal query is not touched by NaN in tokens behind its own; one that sees a NaN value has NaN in that value's column alone, one that sees a
+    NaN key everywhere."""
+    g = _gen(tq + capacity)
+    n = 3
+    cache = _loud_cache(ops, g, n, kv_heads, capacity, d)
+    lens = torch.tensor([capacity, capacity - 37, max(tq, 67)], dtype=torch.int32)
+    for b in range(n):
+        last = int(lens[b]) - 1
+        for h in range(kv_heads):
+            for back, column in ((1, 3 + h), (tq // 3, d - 1), (tq // 2, 17)):
+                if last - back >= 0:
+                    cache[1].view(torch.uint8)[b, h, last - back, column] = 0x7f if h % 2 else 0xff
+            cache[0].view(torch.uint8)[b, h, last, 5] = 0x7f
+    q = torch.randn(n, tq, heads, d, generator=g).to(TYPES[dtype]).cuda()
+    got = ops.kv8_attention(q, *cache, lens.cuda(), causal=True).cpu().double()
+    k, v = (R.values_of(c) * s.cpu().double().repeat_interleave(64, -1)[..., None] for c, s in (cache[::2], cache[1::2]))
+    admitted = torch.arange(capacity) < (lens.long()[:, None] - tq + 1 + torch.arange(tq))[..., None]
+    want, weight, size = R.attention(q, k, v, admitted, d ** -0.5)
+    bound = R.attention_bound(want, weight, size, d, capacity, q.dtype, float(torch.nan_to_num(v).abs().max()))
+    group = heads // kv_heads
+    sees_value = torch.einsum('nik,nhkd->nihd', admitted.double(), v.isnan().double()).repeat_interleave(group, 2) > 0
+    sees_key = torch.einsum('nik,nhk->nih', admitted.double(), k.isnan().any(-1).double()).repeat_interleave(group, 2) > 0
+    lost = sees_value | sees_key[..., None]
+    assert bool(lost.any()) and (tq == 1 or not bool(lost.all()))
+    assert torch.equal(got.isnan(), lost)
+    _close(got.masked_fill(lost, 0), want.masked_fill(lost, 0), bound, 'out')
 
 
 def test_kv8_attention_with_scales_far_apart(ops):

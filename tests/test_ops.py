@@ -92,7 +92,9 @@ REFUSED = [
     ('asr_kv8_append', _append, dict(n=-1)), ('asr_kv8_append', _append, dict(d=24)), ('asr_kv8_append', _append, dict(d=144)),
     ('asr_kv8_append', _append, dict(capacity=65)), ('asr_kv8_append', _append, dict(dtype=3)), ('asr_kv8_append', _append, dict(lens=0)),
     ('asr_kv8_append', _append, dict(k=260)), ('asr_kv8_append', _append, dict(new=2, kst=(64, 62, 64))), ('asr_kv8_append', _append, dict(k8=264)),
-    ('asr_kv8_append', _append, dict(cs=(4100, 4096))), ('asr_kv8_append', _append, dict(n=70000)),
+    ('asr_kv8_append', _append, dict(cs=(4100, 4096))), ('asr_kv8_append', _append, dict(n=70000, v8=1024, vs=512)),
+    ('asr_kv8_append', _append, dict(vs=512)), ('asr_kv8_append', _append, dict(v8=1024)),          # K and V in the same memory
+    ('asr_kv8_append', _append, dict(v8=1024, vs=512, capacity=1 << 23, new=1 << 23)),
     ('asr_kv8_attention', _attend, dict(capacity=65)), ('asr_kv8_attention', _attend, dict(heads=3, kv_heads=2)),
     ('asr_kv8_attention', _attend, dict(d=72)), ('asr_kv8_attention', _attend, dict(dtype=3)), ('asr_kv8_attention', _attend, dict(scale=math.inf)),
     ('asr_kv8_attention', _attend, dict(lens=0)), ('asr_kv8_attention', _attend, dict(v8=0)), ('asr_kv8_attention', _attend, dict(q=260)),
