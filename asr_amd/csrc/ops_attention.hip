@@ -136,6 +136,20 @@ __device__ inline int place_of(int nbh, int per, int64_t& id)
     return bh;
 }
 
+// The sequence that is number `at` when the longest come first (at itself where that would not matter or take too long): the last workgroups of a launch
+// are then short ones (16 x 200 queries over 1500 states of half to full length: 41.5 -> 38 us; one token over 64 caches of up to 2048: 45.7 -> 42.9).  Finding it
+// costs up to half a microsecond a workgroup, too much for few rows over short keys (64 x 10 queries over 334 states: 15.5 -> 16.4 us).
+__device__ inline int longest_first(const AttnArgs& a, int at)
+{
+    if (!a.lens || a.n < 2 || a.n > 64 || a.tk >= 1 << 25) return at;
+    const int lane = threadIdx.x & 63, key = lane < a.n ? keys_of(a, lane) * 64 + 63 - lane : -1;
+    int before = 0;
+    for (int j = 0; j < a.n; j += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) before += __builtin_amdgcn_readlane(key, (j + i) & 63) > key;
+    return __builtin_ctzll(__ballot(lane < a.n && before == at));
+}
+
 // ---- few rows: the waves of a workgroup share the keys ------------------------------------------------------------------
 // A workgroup has one tile of 16 NQ rows of one (sequence, K/V head) and one share of its keys; its four waves take 32 keys at a time in turn,
 // straight from memory into registers in the operands' own order (no LDS in the loop), and join their sums in LDS at the end.  The next chunk's
@@ -202,9 +216,9 @@ void attention_few_kernel(AttnArgs a)
     __shared__ __align__(16) float s_o[FEW_WAVES][16 * NQ][PITCH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x16 = lane & 15, g = lane >> 4;
     int64_t id = blockIdx.x;
-    const int bh = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
+    const int place = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
     const int split = (int)(id % a.nsplit), tile = (int)(id / a.nsplit);
-    const int b = bh / a.kv_heads, h = bh % a.kv_heads;
+    const int b = a.tk >= 1024 ? longest_first(a, place / a.kv_heads) : place / a.kv_heads, h = place % a.kv_heads, bh = b * a.kv_heads + h;
     const int len = keys_of(a, b), row0 = tile * 16 * NQ;
 
     // this tile's keys: all of them, or in a causal call what its last row sees
@@ -577,9 +591,9 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x32 = lane & 31, half = lane >> 5;
 
     int64_t id = blockIdx.x;
-    const int bh = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
+    const int place = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
     const int split = (int)(id % a.nsplit), tile = a.tiles - 1 - (int)(id / a.nsplit);   // (causal: the longest rows first)
-    const int b = bh / a.kv_heads, h = bh % a.kv_heads;
+    const int b = longest_first(a, place / a.kv_heads), h = place % a.kv_heads, bh = b * a.kv_heads + h;
     const int len = keys_of(a, b), row0 = tile * MANY_ROWS;
     int last_key = len;
     if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + MANY_ROWS - 1, a.rows - 1) / a.group + 1));

@@ -245,6 +245,16 @@ def test_cross_attention_strides(ops, tq, dtype):
     assert bool((wide == 5.0).all())
 
 
+@pytest.mark.parametrize('n,tq,kv_heads', [(2, 3, 4), (20, 1, 1), (64, 2, 2), (65, 1, 2), (7, 45, 8), (64, 60, 1)])
+def test_cross_attention_of_many_lengths(ops, n, tq, kv_heads):
+    """Equal, zero and negative lengths and some beyond the end among those of up to 65 sequences, taken in whatever order."""
+    q, kv = _cross_case(n + tq, n, tq, 1100, kv_heads, kv_heads, 64, 'bf16')
+    kv = kv.cuda()
+    lens = torch.randint(-100, 1300, (n,), generator=_gen(n), dtype=torch.int32)
+    lens[n // 2:] = lens[:n - n // 2].flip(0)
+    _check_cross(ops, q.cuda(), kv[:, :, 0], kv[:, :, 1], lens=lens.cuda())
+
+
 def test_cross_attention_without_states_or_queries(ops):
     q = torch.randn(2, 3, 4, 64, device='cuda')
     none = torch.empty(2, 0, 4, 64, device='cuda')
