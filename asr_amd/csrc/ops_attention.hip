@@ -529,13 +529,16 @@ void attention_few_kernel(AttnArgs a)
 }
 
 // ---- many rows: the waves of a workgroup share tiles of keys in LDS ------------------------------------------------------
-// 16-bit products only.  A workgroup has 128 rows, 32 for each of its four waves, and walks over tiles of 64 keys that it stages into LDS (two
-// buffers: the next tile's loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
+// 16-bit products only.  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
+// (K three buffers, V two: the next tiles' loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
 // scale).  32 x 32 x 16 products: S^T = K q^T has a row in each lane of 32 and lane half; O^T = V^T P^T takes V^T from LDS with the transposing read
 // (four keys of one column a lane) and P^T straight from the accumulators, rounded once to the products' type.
 // The 16-byte chunks of a row are permuted by its number (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4), by pairs of rows where rows are half
 // as long): both kinds of read then meet every bank evenly.  Rows of 16-bit values as long as the tile go from memory to LDS directly.
-constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;
+// What bounds it: instructions.  A tile is 32 products (1024 cycles of the matrix pipe) and some 190 vector instructions a wave and row tile; products of one
+// wave run beside the vector instructions of both waves of a SIMD, but a wave alone issues only every 7 cycles.  8 x 768 queries of 32 heads over 4001
+// states of 8 heads of 128: 1000 TFLOP/s while all workgroups run.
+constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;               // (MANY_ROWS: for each row tile of a wave)
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -545,17 +548,17 @@ template <bool F16> __device__ inline f32x16 mfma32(const u32x4& a, const u32x4&
     if (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-__device__ inline u32x2 lds_read_transposed(const char* p)
+__device__ inline u32x2 lds_read_transposed(const __attribute__((address_space(3))) char* p)
 {
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
     return __builtin_bit_cast(u32x2, x);
 }
 // 16 bytes a lane from memory to LDS, the wave's 1024 in lane order from `lds` on; done when the wave has waited for its memory operations.  (The
 // builtin would have every later LDS read wait for it, as the compiler cannot tell the buffers apart.)
-__device__ inline void load_to_lds(mem p, char* lds)
+__device__ inline uint32_t lds_at(char* p) { return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p); }
+__device__ inline void load_to_lds(mem p, uint32_t at)
 {
-    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(at)) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory");
 }
 __device__ inline void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ inline float halves_max(float x)
@@ -576,7 +579,7 @@ template <bool F16> __device__ inline float pair_sum(uint32_t w, float c)
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
 }
 
-template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attention_many_kernel(AttnArgs a)
+template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attention_many_kernel(AttnArgs a)
 {
     constexpr bool F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
     constexpr bool DIRECT = FULL && !CODES;
@@ -584,8 +587,8 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     constexpr int ROW_LOADS = DP / (CODES ? 16 : 8);                            // 16-byte loads of a key row
     constexpr int LOADS = MANY_KEYS * ROW_LOADS / (64 * MANY_WAVES);              // of a thread, for K and for V
     constexpr int LOAD_ROWS = 64 * MANY_WAVES / ROW_LOADS;                        // rows from one load of a thread to its next (a multiple of 16)
-    __shared__ __align__(16) char s_k[3][MANY_KEYS * PITCH];
-    __shared__ __align__(16) char s_v[2][MANY_KEYS * PITCH];
+    __shared__ __align__(16) char s_kv[5][MANY_KEYS * PITCH];
+    char(*const s_k)[MANY_KEYS * PITCH] = s_kv, (*const s_v)[MANY_KEYS * PITCH] = s_kv + 3;
     const auto turn_k = [](int row) { return (row / PAIR) & (DP / 8 - 1); };                 // of a row's 16-byte chunks
     const auto turn_v = [](int row) { return PAIR == 1 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x32 = lane & 31, half = lane >> 5;
@@ -594,26 +597,30 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     const int place = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
     const int split = (int)(id % a.nsplit), tile = a.tiles - 1 - (int)(id / a.nsplit);   // (causal: the longest rows first)
     const int b = longest_first(a, place / a.kv_heads), h = place % a.kv_heads, bh = b * a.kv_heads + h;
-    const int len = keys_of(a, b), row0 = tile * MANY_ROWS;
+    const int len = keys_of(a, b), row0 = tile * MANY_ROWS * NR, wave_row0 = row0 + 32 * NR * wave;
     int last_key = len;
-    if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + MANY_ROWS - 1, a.rows - 1) / a.group + 1));
+    if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + MANY_ROWS * NR - 1, a.rows - 1) / a.group + 1));
     const int first_lim = a.causal ? len - a.tq + row0 / a.group + 1 : 0x7fffffff;       // every row of this workgroup sees the keys below it
     const int all_tiles = (last_key + MANY_KEYS - 1) / MANY_KEYS, share = (all_tiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * share, t1 = min(all_tiles, t0 + share);
 
     // q as second operand (a negative factor is moved into it: exact)
-    const int r = row0 + 32 * wave + x32, rc = min(r, a.rows - 1);
-    const char* qp = a.q + (int64_t)b * a.q_stride[0] + (int64_t)(rc / a.group) * a.q_stride[1] + (int64_t)(h * a.group + rc % a.group) * a.q_stride[2];
     const float c = fmaxf(fabsf(a.c), 1e-37f);                                        // (a factor of 0 must leave -infinity what it is)
-    u32x4 qf[DP / 16];
+    u32x4 qf[NR][DP / 16];
+    int lim[NR];                                                                      // this lane's rows see keys below it
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u) {
-        const int at = 16 * u + 8 * half;
-        qf[u] = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
-        if (a.c < 0) qf[u] ^= 0x80008000u;
+    for (int t = 0; t < NR; ++t) {
+        const int r = wave_row0 + 32 * t + x32, rc = min(r, a.rows - 1);
+        const char* qp = a.q + (int64_t)b * a.q_stride[0] + (int64_t)(rc / a.group) * a.q_stride[1] + (int64_t)(h * a.group + rc % a.group) * a.q_stride[2];
+#pragma unroll
+        for (int u = 0; u < DP / 16; ++u) {
+            const int at = 16 * u + 8 * half;
+            qf[t][u] = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
+            if (a.c < 0) qf[t][u] ^= 0x80008000u;
+        }
+        lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
     }
-    const int lim = a.causal ? len - a.tq + rc / a.group + 1 : len;                 // this lane's row sees keys below it
-    const int wave_first = a.causal ? len - a.tq + min(row0 + 32 * wave, a.rows - 1) / a.group + 1 : 0x7fffffff;      // every row of this wave sees keys below it
+    const int wave_first = a.causal ? len - a.tq + min(wave_row0, a.rows - 1) / a.group + 1 : 0x7fffffff;      // every row of this wave sees keys below it
 
     const char* kb = a.k + (int64_t)b * a.k_stride[0] + (int64_t)h * a.k_stride[2];
     const char* vb = a.v + (int64_t)b * a.v_stride[0] + (int64_t)h * a.v_stride[2];
@@ -653,10 +660,13 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
         }
     };
     // ... load u of them, to registers or LDS
-    const auto load = [&](const mem (&x)[LOADS], int u, u32x4* regs, char* lds) __attribute__((always_inline)) {
-        if constexpr (DIRECT) load_to_lds(x[u], lds + (u * MANY_WAVES + wave) * 1024);
+    const auto load = [&](const mem (&x)[LOADS], int u, u32x4* regs, uint32_t lds) __attribute__((always_inline)) {
+        if constexpr (DIRECT) load_to_lds(x[u], lds + u * MANY_WAVES * 1024);
         else regs[u] = load_as<u32x4>(x[u]);
     };
+    const uint32_t my_lds = lds_at(s_k[0]) + wave * 1024, tile_bytes = MANY_KEYS * PITCH;                       // where this wave's loads of K go, of V behind them
+    const auto k_lds = [&](int buf) { return my_lds + buf * tile_bytes; };
+    const auto v_lds = [&](int t) { return my_lds + (3 + (t & 1)) * tile_bytes; };
     // fetched registers into LDS (the caller waits and meets the other waves afterwards)
     const auto put = [&](u32x4* regs, char* lds, float scale, auto turn) __attribute__((always_inline)) {
 #pragma unroll
@@ -722,128 +732,170 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
     // 16 (group % 2) + 0 .. 15, its lane i key i / 4 and four columns from 4 (i % 4)
     const int k_read = x32 * PITCH + 16 * (half ^ turn_k(x32)), v_row = 4 * half + ((lane & 15) >> 2);
     const int v_read = v_row * PITCH + 8 * (lane & 1) + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ turn_v(v_row));
-    f32x16 o[DP / 32];
+    f32x16 o[NR][DP / 32];
+    float m[NR], l[NR], top[NR];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
-    float m = NO_MAX, l = 0.0f;
+    for (int t = 0; t < NR; ++t) {
+        m[t] = NO_MAX;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) o[t][i] = f32x16{};
+    }
     uint64_t mask = 0;
-    constexpr int AHEAD = 4, N = DP / 16, PAIRS = 8 / N;                             // N products of a half's scores, and of its output
+    constexpr int AHEAD = 4, N = DP / 16;                                            // N products of a half's scores, and of its output, for each row tile
     u32x4 kf[N];                                                                     // of the next half's scores, AHEAD of them read beforehand
 
-    const auto scores = [&](const char* k_tile, int sub, f32x16& s) __attribute__((always_inline)) {
-        s = f32x16{};
-#pragma unroll
-        for (int u = 0; u < DP / 16; ++u) s = mfma32<F16>(*reinterpret_cast<const u32x4*>(k_tile + 32 * sub * PITCH + (k_read ^ (32 * u))), qf[u], s);
+    // LDS addresses of the reads, renewed when a tile is first read (its halves differ by a constant in the instruction)
+    typedef const __attribute__((address_space(3))) char* lds_mem;
+    const lds_mem kv_lds = (lds_mem)s_kv[0];
+    lds_mem kf_at[N], vf_at[N / 2];
+    const auto k_frag = [&](int buf, int sub, int u) __attribute__((always_inline)) {
+        if (sub == 0) {
+            kf_at[u] = kv_lds + buf * (MANY_KEYS * PITCH) + (k_read ^ (32 * u));
+            asm volatile("" : "+v"(kf_at[u]));
+        }
+        return *(const __attribute__((address_space(3))) u32x4*)(kf_at[u] + 32 * sub * PITCH);
     };
-    const auto k_frag = [&](const char* k_half, int u) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4*>(k_half + (k_read ^ (32 * u))); };
+    const auto score = [&](const u32x4& k, int r, int u, f32x16& s) __attribute__((always_inline)) {
+        s = mfma32<F16>(k, qf[r][u], u == 0 ? f32x16{} : s);
+    };
     const auto most = [&](const f32x16& s) __attribute__((always_inline)) {
-        float top = s[0];
+        float x = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        return halves_max(top) * c;
+        for (int i = 1; i < 16; ++i) x = fmaxf(x, s[i]);
+        return halves_max(x) * c;
     };
-    // soft-max and output of half `sub` of tile t from its scores s with their maximum `top`, and the scores of the half behind it: the matrix pipe
-    // computes those while the exponentials run, and the output while their maximum is taken.  The next tiles' loads go out one at a time in between
-    // (all at once they fill the memory pipe's queue and the wave waits: 1060 of 3500 cycles a tile).
-    const auto step = [&](int t, int sub, f32x16& s, float& top, const char* next_tile, const char* k_half_after, f32x16& next, const mem (&from)[LOADS], u32x4* regs,
-                          char* to) __attribute__((always_inline)) {
+    uint64_t grow = 0;                                                               // the lanes whose rows' maximum has grown
+    const auto grows = [&]() __attribute__((always_inline)) {
+        bool x = top[0] > m[0] + SLACK;
+        if (NR > 1) x |= top[NR - 1] > m[NR - 1] + SLACK;
+        return __ballot(x);
+    };
+    // soft-max and output of half `sub` of tile t from its scores s with their maxima `top`, and the scores of the half behind it.  The products are laid out
+    // as slots, one for each, and between them, in the order in which it is to be issued (the compiler left to itself puts all products on one
+    // side): the LDS reads AHEAD products before their own; the exponentials, over the slots of the scores and of the output's first half, whose probabilities
+    // the second half multiplies - each value a stage further a slot later, so that none waits for the one before; the maxima of the new scores; and
+    // the next tiles' loads, one a slot (all at once they fill the memory pipe's queue and the wave waits).
+    const auto step = [&](int t, int sub, f32x16 (&s)[NR], int next_buf, int buf_after, f32x16 (&next)[NR], auto bring) __attribute__((always_inline)) {
         const int c0 = t * MANY_KEYS + 32 * sub;
         const uint32_t bits = (uint32_t)(mask >> (32 * sub));
         if (bits != ~0u || c0 + 32 > wave_first) {
             asm volatile("");                                                       // (a branch, not 16 selects in every step)
             const uint32_t mine = bits >> (4 * half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = admit(s[i], spread_bit(mine, 8 * (i >> 2) + (i & 3)));
-            if (c0 + 32 > wave_first) {                                             // (causal calls)
-                asm volatile("");
+            for (int r = 0; r < NR; ++r) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = c0 + 8 * (i >> 2) + 4 * half + (i & 3) < lim ? s[i] : NEG_INF;
+                for (int i = 0; i < 16; ++i) s[r][i] = admit(s[r][i], spread_bit(mine, 8 * (i >> 2) + (i & 3)));
+                if (c0 + 32 > wave_first) {                                         // (causal calls)
+                    asm volatile("");
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[r][i] = c0 + 8 * (i >> 2) + 4 * half + (i & 3) < lim[r] ? s[r][i] : NEG_INF;
+                }
+                top[r] = most(s[r]);
             }
-            top = most(s);
+            grow = grows();
         }
-        if (__ballot(top > m + SLACK)) {
-            const float grown = fmaxf(m, top), f = rescale(m, grown);
-            m = grown;
-            l *= f;
+        if (grow) {
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i)
+            for (int r = 0; r < NR; ++r) {
+                const float grown = top[r] > m[r] + SLACK ? top[r] : m[r], f = rescale(m[r], grown);
+                m[r] = grown;
+                l[r] *= f;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[i][j] *= f;
+                for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[r][i][j] *= f;
+            }
         }
-        // In the order in which it is to be issued (the compiler left to itself puts all products on one side): an LDS read AHEAD products before its own
-        // product, between the products their share of the exponentials - each value a stage further a product later, so that none waits for the
-        // one before - then of the maximum
-        const char *k_half = next_tile + 32 * (sub ^ 1) * PITCH, *v_half = s_v[t & 1] + 32 * sub * PITCH;
         const auto v_frag = [&](int q) __attribute__((always_inline)) {
-            const char* p = v_half + 16 * (q / (N / 2)) * PITCH + (v_read ^ (64 * (q % (N / 2))));
+            const int i = q % (N / 2);
+            if (sub == 0 && q < N / 2) {
+                vf_at[i] = kv_lds + (3 + (t & 1)) * (MANY_KEYS * PITCH) + (v_read ^ (64 * i));
+                asm volatile("" : "+v"(vf_at[i]));
+            }
+            const lds_mem p = vf_at[i] + (32 * sub + 16 * (q / (N / 2))) * PITCH;
             const u32x2 lo = lds_read_transposed(p), hi = lds_read_transposed(p + 8 * PITCH);
             return u32x4{lo[0], lo[1], hi[0], hi[1]};
         };
+        constexpr int SLOTS = N * NR, VALUES = 16 * NR, FROM = SLOTS / 4 < 2 ? 1 : SLOTS / 2 - 2 < 2 ? SLOTS / 2 - 2 : 2;
         u32x4 vf[N];
-        float x[16];
-        uint32_t pf[8];
-        float sum = 0.0f;
-        next = f32x16{};
+        float x[NR][16], most_of[NR][2];
+        uint32_t pf[NR][8];
+        // value e in the order in which they are needed: the first 16 keys' of every row tile, then the others'
+        const auto row_of = [](int e) { return e / 8 % NR; };
+        const auto key_of = [](int e) { return 8 * (e / (8 * NR)) + e % 8; };
+        // values whose exponential is taken by the end of slot w: all before the output's second half
+        const auto taken = [](int w) { return w < 0 ? 0 : VALUES * (w + 1) >= VALUES * (SLOTS * 3 / 2 - 1) ? VALUES : (VALUES * (w + 1) + SLOTS * 3 / 2 - 2) / (SLOTS * 3 / 2 - 1); };
+        const auto begin = [&](int e) __attribute__((always_inline)) { x[row_of(e)][key_of(e)] = fmaf(s[row_of(e)][key_of(e)], c, -m[row_of(e)]); };
+        const auto between = [&](int w) __attribute__((always_inline)) {
+            if (w >= SLOTS * 3 / 2) return;
 #pragma unroll
-        for (int j = 0; j < 2 * PAIRS; ++j) x[j] = fmaf(s[j], c, -m);
+            for (int e = taken(w); e < taken(w + 1); ++e) begin(e);
+#pragma unroll
+            for (int e = taken(w - 1); e < taken(w); ++e) x[row_of(e)][key_of(e)] = __builtin_amdgcn_exp2f(x[row_of(e)][key_of(e)]);
+#pragma unroll
+            for (int i = taken(w - 2) / 2; i < taken(w - 1) / 2; ++i) {
+                const int r = row_of(2 * i), j = key_of(2 * i);
+                pf[r][j / 2] = pack16<F16>(x[r][j], x[r][j + 1]);
+                l[r] = pair_sum<F16>(pf[r][j / 2], l[r]);
+            }
+        };
+#pragma unroll
+        for (int e = 0; e < taken(0); ++e) begin(e);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            if (u + AHEAD < N) kf[u + AHEAD] = k_frag(k_half, u + AHEAD);
-            else vf[u + AHEAD - N] = v_frag(u + AHEAD - N);
-            next = mfma32<F16>(kf[u], qf[u], next);
-            if (u % (N / LOADS) == 0 && u / (N / LOADS) < LOADS) load(from, u / (N / LOADS), regs, to);
+        for (int w = 0; w < SLOTS; ++w) {
+            const int u = w / NR, r = w % NR;
+            if (r == 0) {
+                if (u + AHEAD < N) kf[u + AHEAD] = k_frag(next_buf, sub ^ 1, u + AHEAD);
+                else vf[u + AHEAD - N] = v_frag(u + AHEAD - N);
+            }
+            score(kf[u], r, u, next[r]);
+            bring(w);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int j = 2 * PAIRS * u; j < 2 * PAIRS * (u + 1); ++j) {
-                if (j + 2 * PAIRS < 16) x[j + 2 * PAIRS] = fmaf(s[j + 2 * PAIRS], c, -m);
-                x[j] = __builtin_amdgcn_exp2f(x[j]);
-            }
-            if (u > 0) {
-#pragma unroll
-                for (int i = PAIRS * (u - 1); i < PAIRS * u; ++i) {
-                    pf[i] = pack16<F16>(x[2 * i], x[2 * i + 1]);
-                    sum = pair_sum<F16>(pf[i], sum);
-                }
-            }
+            between(w);
             __builtin_amdgcn_sched_barrier(0);
         }
-        float most_of[2];
 #pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const int k16 = q / (N / 2), i = q % (N / 2);
-            if (q + AHEAD < N) vf[q + AHEAD] = v_frag(q + AHEAD);
-            else kf[q + AHEAD - N] = k_frag(k_half_after, q + AHEAD - N);
-            if (q == 0) {
-#pragma unroll
-                for (int j = PAIRS * (N - 1); j < 8; ++j) {
-                    pf[j] = pack16<F16>(x[2 * j], x[2 * j + 1]);
-                    sum = pair_sum<F16>(pf[j], sum);
-                }
+        for (int w = 0; w < SLOTS; ++w) {
+            const int q = w / NR, r = w % NR, k16 = q / (N / 2), i = q % (N / 2);
+            if (r == 0) {
+                if (q + AHEAD < N) vf[q + AHEAD] = v_frag(q + AHEAD);
+                else kf[q + AHEAD - N] = k_frag(buf_after, sub, q + AHEAD - N);
             }
-            o[i] = mfma32<F16>(vf[q], u32x4{pf[4 * k16], pf[4 * k16 + 1], pf[4 * k16 + 2], pf[4 * k16 + 3]}, o[i]);
+            o[r][i] = mfma32<F16>(vf[q], u32x4{pf[r][4 * k16], pf[r][4 * k16 + 1], pf[r][4 * k16 + 2], pf[r][4 * k16 + 3]}, o[r][i]);
+            bring(SLOTS + w);
             __builtin_amdgcn_sched_barrier(0);
-            if (q == N / 2) {
-                most_of[0] = next[0];
-                most_of[1] = next[1];
-            }
-            if (q >= N / 2) {
+            between(SLOTS + w);
+            if (w >= FROM && w < FROM + SLOTS / 2) {
 #pragma unroll
-                for (int j = 32 * (q - N / 2) / N; j < 32 * (q + 1 - N / 2) / N; j += 4) {
-                    most_of[0] = fmaxf(fmaxf(most_of[0], next[j]), next[j + 2]);
-                    most_of[1] = fmaxf(fmaxf(most_of[1], next[j + 1]), next[j + 3]);
+                for (int e = VALUES * (w - FROM) / (SLOTS / 2); e < VALUES * (w + 1 - FROM) / (SLOTS / 2); e += 2) {
+                    float(&y)[2] = most_of[e / 16];
+                    const f32x16& z = next[e / 16];
+                    if (e % 16 == 0) y[0] = z[0], y[1] = z[1];
+                    else if (e % 4 == 0) y[0] = fmaxf(fmaxf(y[0], z[e % 16]), z[e % 16 + 1]);
+                    else y[1] = fmaxf(fmaxf(y[1], z[e % 16]), z[e % 16 + 1]);
                 }
-                asm volatile("" : "+v"(most_of[0]), "+v"(most_of[1]));                  // (here, not behind the last product)
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+                    if (VALUES * (w + 1 - FROM) / (SLOTS / 2) > 16 * r + 3 && VALUES * (w - FROM) / (SLOTS / 2) < 16 * (r + 1))
+                        asm volatile("" : "+v"(most_of[r][0]), "+v"(most_of[r][1]));                  // (here, not behind the last product)
             }
+            if (w == FROM + SLOTS / 2) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    top[r] = halves_max(fmaxf(most_of[r][0], most_of[r][1])) * c;
+                    asm volatile("" : "+v"(top[r]));
+                }
+            }
+            if (w == SLOTS - 1) grow = grows();
             __builtin_amdgcn_sched_barrier(0);
         }
-        l += sum;
-        top = halves_max(fmaxf(most_of[0], most_of[1])) * c;
     };
 
     if (t0 < t1) {
-        f32x16 sa, sb;
-        mem from[LOADS];
+        f32x16 sa[NR], sb[NR];
+        mem from[LOADS], v_places[LOADS];
         int now = 0, behind = 1, fetched = 2;                                           // K buffers of tiles t, t + 1, t + 2
         mask = admitted(t0, flag_of(t0));
         // this thread's first row of the tile that is loaded next
@@ -853,24 +905,29 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
             aim(t, k_from, a.k_stride[1], k_step, from);
             if constexpr (CODES) ks = ksc[t];
 #pragma unroll
-            for (int u = 0; u < LOADS; ++u) load(from, u, kr, s_k[buf]);
+            for (int u = 0; u < LOADS; ++u) load(from, u, kr, k_lds(buf));
             put_k(buf);
         };
         bring_k(t0, now);
         aim(t0, v_from, a.v_stride[1], v_step, from);
         if constexpr (CODES) vs = vsc[t0];
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) load(from, u, vr, s_v[t0 & 1]);
+        for (int u = 0; u < LOADS; ++u) load(from, u, vr, v_lds(t0));
         put_v(t0, mask);
         if (t0 + 1 < t1) {
             k_from += k_tile;
             bring_k(t0 + 1, behind);
         }
         meet();
-        scores(s_k[now], 0, sa);
-        float top = most(sa);
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) kf[u] = k_frag(s_k[now] + 32 * PITCH, u);
+        for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) score(k_frag(now, 0, u), r, u, sa[r]);
+            top[r] = most(sa[r]);
+        }
+        grow = grows();
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) kf[u] = k_frag(now, 1, u);
         for (int t = t0; t < t1; ++t) {
             // (behind the last tile the last one is loaded again, and scores are taken of what LDS holds: neither is used)
             const int tk = min(t + 2, t1 - 1), tv = min(t + 1, t1 - 1);
@@ -878,11 +935,17 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
             if (t + 2 < t1) k_from += k_tile;
             if (t + 1 < t1) v_from += v_tile;
             aim(tk, k_from, a.k_stride[1], k_step, from);
-            if constexpr (CODES) ks = ksc[tk];
-            step(t, 0, sa, top, s_k[now], s_k[behind], sb, from, kr, s_k[fetched]);
-            aim(tv, v_from, a.v_stride[1], v_step, from);
-            if constexpr (CODES) vs = vsc[tv];
-            step(t, 1, sb, top, s_k[behind], s_k[behind] + 32 * PITCH, sa, from, vr, s_v[(t + 1) & 1]);
+            aim(tv, v_from, a.v_stride[1], v_step, v_places);
+            if constexpr (CODES) {
+                ks = ksc[tk];
+                vs = vsc[tv];
+            }
+            step(t, 0, sa, now, behind, sb, [&](int w) __attribute__((always_inline)) {
+                if (w % NR) return;
+                if (w / NR < LOADS) load(v_places, w / NR, vr, v_lds(t + 1));
+                else if (w / NR < 2 * LOADS) load(from, w / NR - LOADS, kr, k_lds(fetched));
+            });
+            step(t, 1, sb, behind, behind, sa, [](int) {});
             if (t + 1 < t1) {
                 put_k(fetched);
                 mask = admitted(t + 1, next_flag);
@@ -903,8 +966,7 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
                 __syncthreads();
                 if (waves[0] | waves[1] | waves[2] | waves[3]) {
                     // where this lane's row sees a NaN its sum is one
-                    const int to = min(t1 * MANY_KEYS, lim);
-                    for (int key = max(t0, first_lim >> 6) * MANY_KEYS; key < to; ++key)
+                    for (int key = max(t0, first_lim >> 6) * MANY_KEYS; key < min(t1 * MANY_KEYS, len); ++key)
 #pragma unroll
                         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -912,40 +974,47 @@ template <int QT, int KVT, int DP, bool FULL> __global__ __launch_bounds__(64 * 
                                 const int at = 32 * i + 8 * j + 4 * half;
                                 const uint32_t x = at < a.d ? nan_codes(load_as<uint32_t>((mem)vb + (int64_t)key * a.v_stride[1] + at)) : 0u;
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) o[i][4 * j + e] = (x >> (8 * e)) & 1 ? __builtin_nanf("") : o[i][4 * j + e];
+                                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                    for (int r = 0; r < NR; ++r)
+                                        o[r][i][4 * j + e] = key < lim[r] && (x >> (8 * e)) & 1 ? __builtin_nanf("") : o[r][i][4 * j + e];
                             }
                 }
             }
         }
     }
 
-    if (r >= a.rows) return;
-    const float sum = halves_sum(l);
-    if (a.nsplit > 1) {
-        float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
-        if (half == 0) { ws[0] = m; ws[1] = sum; }
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        const int r = wave_row0 + 32 * t + x32;
+        const float sum = halves_sum(l[t]);
+        if (r >= a.rows) continue;
+        if (a.nsplit > 1) {
+            float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
+            if (half == 0) { ws[0] = m[t]; ws[1] = sum; }
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = 32 * i + 8 * j + 4 * half;
+                    if (at < a.d) *reinterpret_cast<f32x4*>(ws + 4 + at) = f32x4{o[t][i][4 * j], o[t][i][4 * j + 1], o[t][i][4 * j + 2], o[t][i][4 * j + 3]};
+                }
+            continue;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] + (int64_t)(h * a.group + r % a.group) * a.out_stride[2];
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int at = 32 * i + 8 * j + 4 * half;
-                if (at < a.d) *reinterpret_cast<f32x4*>(ws + 4 + at) = f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+                if (at >= a.d) continue;
+                u32x2 w;
+                w[0] = pack16<QT == ASR_F16>(o[t][i][4 * j] * inv, o[t][i][4 * j + 1] * inv);
+                w[1] = pack16<QT == ASR_F16>(o[t][i][4 * j + 2] * inv, o[t][i][4 * j + 3] * inv);
+                *reinterpret_cast<u32x2*>(op + 2 * at) = w;
             }
-        return;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    char* op = a.out + (int64_t)b * a.out_stride[0] + (int64_t)(r / a.group) * a.out_stride[1] + (int64_t)(h * a.group + r % a.group) * a.out_stride[2];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = 32 * i + 8 * j + 4 * half;
-            if (at >= a.d) continue;
-            u32x2 w;
-            w[0] = pack16<QT == ASR_F16>(o[i][4 * j] * inv, o[i][4 * j + 1] * inv);
-            w[1] = pack16<QT == ASR_F16>(o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv);
-            *reinterpret_cast<u32x2*>(op + 2 * at) = w;
-        }
 }
 
 // Joins the shares of a long key axis.  A row has 32 G threads: four values each, every G-th share (a row's shares are far apart, so the loads of many
@@ -1012,7 +1081,12 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
     p.rows = (int)(tq * (heads / kv_heads));
     p.many = sixteen && p.rows > 40;            // (48 rows of 64 over 1000 states: 51 us and 55 with the other, 40 rows: 23 and 20)
     if (p.many) {
-        p.tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
+        // two row tiles a wave where its registers hold them and workgroups of twice the rows still give every compute unit two, without many idle rows (8 x 512
+        // queries of 32 heads over 4096 states of 8 heads of 64: 174 us with one, 156 with two, half of them 92 and 88; heads of 128 would leave one wave a SIMD: 152
+        // and 160)
+        const int64_t tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
+        p.nq = d == 64 && (tiles % 2 == 0 || tiles >= 8) && n * kv_heads * ((tiles + 1) / 2) >= 512 ? 2 : 1;
+        p.tiles = (int)((tiles + p.nq - 1) / p.nq);
         const int64_t wgs = n * kv_heads * p.tiles, most = tk / (MANY_KEYS * 8);
         int64_t split = wgs > 0 ? 512 / wgs : 1;
         if (split > most) split = most;
@@ -1043,12 +1117,12 @@ template <int QT, int KVT> hipError_t launch_few(const AttnArgs& a, int nq, hipS
     return nq == 1 ? ops_launch(attention_few_kernel<QT, KVT, 128, 1, false>, grid, block, s, a) : ops_launch(attention_few_kernel<QT, KVT, 128, 2, false>, grid, block, s, a);
 }
 
-template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, hipStream_t s)
+template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, int nr, hipStream_t s)
 {
     const dim3 grid((uint32_t)((int64_t)a.n * a.kv_heads * a.nsplit * a.tiles)), block(64 * MANY_WAVES);
-    if (a.d == 64) return ops_launch(attention_many_kernel<QT, KVT, 64, true>, grid, block, s, a);
-    if (a.d == 128) return ops_launch(attention_many_kernel<QT, KVT, 128, true>, grid, block, s, a);
-    return a.d < 64 ? ops_launch(attention_many_kernel<QT, KVT, 64, false>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 128, false>, grid, block, s, a);
+    if (a.d == 64) return nr == 2 ? ops_launch(attention_many_kernel<QT, KVT, 64, 2, true>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 64, 1, true>, grid, block, s, a);
+    if (a.d == 128) return ops_launch(attention_many_kernel<QT, KVT, 128, 1, true>, grid, block, s, a);
+    return a.d < 64 ? ops_launch(attention_many_kernel<QT, KVT, 64, 1, false>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 128, 1, false>, grid, block, s, a);
 }
 
 template <int QT> hipError_t launch_join(const AttnArgs& a, hipStream_t s)
@@ -1069,7 +1143,7 @@ template <int QT, int KVT> int attend(const char* what, AttnArgs& a, const Plan&
         a.ws = static_cast<float*>(ws);
     }
     hipError_t e;
-    if constexpr (QT != ASR_F32 && !(QT == ASR_F16 && KVT == KV_E4M3)) e = p.many ? launch_many<QT, KVT>(a, s) : launch_few<QT, KVT>(a, p.nq, s);
+    if constexpr (QT != ASR_F32 && !(QT == ASR_F16 && KVT == KV_E4M3)) e = p.many ? launch_many<QT, KVT>(a, p.nq, s) : launch_few<QT, KVT>(a, p.nq, s);
     else e = launch_few<QT, KVT>(a, p.nq, s);
     if (e == hipSuccess && p.nsplit > 1) e = launch_join<QT>(a, s);
     return ops_launched(what, e);

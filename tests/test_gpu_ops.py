@@ -255,6 +255,25 @@ def test_cross_attention_of_many_lengths(ops, n, tq, kv_heads):
     _check_cross(ops, q.cuda(), kv[:, :, 0], kv[:, :, 1], lens=lens.cuda())
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('n,tq,tk,heads,kv_heads', [(64, 200, 130, 8, 8), (4, 520, 65, 256, 128), (64, 129, 64, 8, 8), (3, 1030, 90, 64, 64)])
+def test_cross_attention_of_many_rows_and_sequences(ops, n, tq, tk, heads, kv_heads, dtype):
+    q, kv = _cross_case(n + tq, n, tq, tk, heads, kv_heads, 64, dtype)
+    lens = torch.randint(0, tk + 1, (n,), generator=_gen(n), dtype=torch.int32)
+    pad = torch.rand(n, tk, generator=_gen(tq)) < 0.2
+    kv = kv.cuda()
+    _check_cross(ops, q.cuda(), kv[:, :, 0], kv[:, :, 1], lens=lens.cuda(), pad=pad.cuda())
+
+
+@pytest.mark.parametrize('causal', [False, True])
+def test_kv8_attention_of_many_rows_and_sequences(ops, causal):
+    g = _gen(9)
+    cache = _loud_cache(ops, g, 64, 8, 256, 64)
+    q = torch.randn(64, 130, 16, 64, generator=g).bfloat16().cuda()
+    lens = torch.randint(100, 257, (64,), generator=g, dtype=torch.int32)
+    _check_kv8(ops, q, cache, lens.cuda(), causal=causal)
+
+
 def test_cross_attention_without_states_or_queries(ops):
     q = torch.randn(2, 3, 4, 64, device='cuda')
     none = torch.empty(2, 0, 4, 64, device='cuda')
@@ -477,7 +496,8 @@ def test_kv8_attention_lengths(ops, tq, heads, kv_heads, d, causal, dtype):
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
 @pytest.mark.parametrize('tq,heads,kv_heads,capacity,d', [(1, 2, 2, 128, 64), (9, 4, 2, 192, 128), (24, 2, 1, 128, 80), (8, 2, 2, 2048, 64), (90, 2, 2, 192, 128),
-                                                          (150, 4, 2, 320, 64), (70, 2, 1, 128, 48), (200, 1, 1, 2048, 128)])
+                                                          (150, 4, 2, 320, 64), (70, 2, 1, 128, 48), (200, 1, 1, 2048, 128),
+                                                          (140, 172, 172, 192, 64)])
 def test_kv8_attention_nan_in_later_tokens(ops, tq, heads, kv_heads, capacity, d, dtype):
     """A causal query is not touched by NaN in tokens behind its own; one that sees a NaN value has NaN in that value's column alone, one that sees a
     NaN key everywhere."""
@@ -488,7 +508,7 @@ def test_kv8_attention_nan_in_later_tokens(ops, tq, heads, kv_heads, capacity, d
     for b in range(n):
         last = int(lens[b]) - 1
         for h in range(kv_heads):
-            for back, column in ((1, 3 + h), (tq // 3, d - 1), (tq // 2, 17)):
+            for back, column in ((1, (3 + h) % d), (tq // 3, d - 1), (tq // 2, 17)):
                 if last - back >= 0:
                     cache[1].view(torch.uint8)[b, h, last - back, column] = 0x7f if h % 2 else 0xff
             cache[0].view(torch.uint8)[b, h, last, 5] = 0x7f
