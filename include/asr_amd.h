@@ -296,7 +296,8 @@ const char* asr_ops_last_error(void);
  * A negative token stands for "no token" (padding): its log probability is 0.  A token >= vocab gives NaN.  Logits of -infinity
  * are masked-out tokens (p = 0, no share in the entropy); a row with nothing else gives log p = -infinity and entropy 0.  A row with a NaN or
  * +infinity gives NaN throughout (its top_tokens are valid token numbers, no more).
- * Everything is computed in float32.  model.py:345-360 has the pieces: log_softmax + top_k of test_output, the cross entropy of test_loss. */
+ * Everything is computed in float32; where a row starts within 16 bytes groups its sums, so the same row elsewhere may differ in a last bit.
+ * model.py:345-360 has the pieces: log_softmax + top_k of test_output, the cross entropy of test_loss. */
 typedef struct asr_token_logprobs_args {
     const void* logits;
     const void* tokens;                  /* [rows] int32 or int64 */

@@ -624,6 +624,68 @@ def test_captured_and_replayed(ops, tk):
             assert bool(torch.isfinite(eager[2]).all())
 
 
+def test_calls_on_two_streams_at_once(ops):
+    """Long keys (a workspace each) and many rows, queued on two streams in turn: each gives what it gives alone."""
+    states = [_together(ops, 50 + i, tk=7000) for i in range(2)]
+    for s in states:
+        s['elens'] = torch.tensor([7000, 6999, 3000], dtype=torch.int32).cuda()
+    many = [torch.randn(2, 300, 8, 64, generator=_gen(60 + i)).bfloat16().cuda() for i in range(2)]
+    long = [torch.randn(2, 1500, 2, 8, 64, generator=_gen(70 + i)).bfloat16().cuda() for i in range(2)]
+
+    def run(i):
+        ctx = ops.cross_attention(many[i], long[i][:, :, 0], long[i][:, :, 1])
+        return [ctx] + list(_step(ops, dict(states[i], cache=[c.clone() for c in states[i]['cache']])))
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for turn in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append((i, run(i)))
+    torch.cuda.synchronize()
+    for i, out in got:
+        for x, y in zip(out, want[i]):
+            assert torch.equal(x, y)
+
+
+def test_lengths_and_counts_at_the_ends_of_int32(ops):
+    g = _gen(80)
+    low, high = -2 ** 31, 2 ** 31 - 1
+    lens = torch.tensor([low, high, 5, 0], dtype=torch.int32)
+    q, kv = _cross_case(80, 4, 3, 130, 2, 2, 64, 'bf16')
+    kv = kv.cuda()
+    _check_cross(ops, q.cuda(), kv[:, :, 0], kv[:, :, 1], lens=lens.cuda())
+    cache = _loud_cache(ops, g, 4, 2, 128, 64)
+    for causal in (False, True):
+        _check_kv8(ops, q.cuda(), cache, lens.cuda(), causal=causal)
+    k, v = (torch.randn(4, 3, 2, 64, generator=g).cuda() for _ in range(2))
+    cache = _random_cache(ops, g, 4, 2, 128, 64)
+    _check_append(ops, k, v, cache, torch.tensor([low, high, 5, 0], dtype=torch.int32).cuda(), torch.tensor([3, 3, high, low], dtype=torch.int32).cuda())
+
+
+def test_more_rows_and_sequences_than_one_grid_dimension(ops):
+    rows = (1 << 20) + 9
+    logits = torch.randn(rows, 5, generator=_gen(90)).half().cuda()
+    tokens = torch.randint(-1, 5, (rows,), generator=_gen(91)).cuda()
+    logp, entropy, top_logp, top_tokens = ops.token_logprobs(logits, tokens, top=2)
+    some = torch.cat([torch.arange(50), torch.arange(rows - 50, rows)]).cuda()
+    # (against 64 bits, not against a call on these rows alone: where a row starts within 16 bytes groups its sums)
+    want_lp, want_h, want_tops, want_at = R.token_logprobs(logits[some], tokens[some].cpu(), 2)
+    bound = R.logprob_bound(logits[some])
+    _close(logp[some], want_lp, bound, 'log p')
+    _close(entropy[some], want_h, bound * (1 + want_h), 'entropy')
+    _close(top_logp[some], want_tops, bound[:, None], 'alternatives')
+    assert torch.equal(top_tokens[some].cpu().long(), want_at)
+    n = 70001
+    q, kv = torch.randn(n, 1, 1, 8, generator=_gen(92)).cuda(), torch.randn(n, 3, 2, 1, 8, generator=_gen(93)).cuda()
+    lens = torch.randint(0, 4, (n,), generator=_gen(94), dtype=torch.int32).cuda()
+    out = ops.cross_attention(q, kv[:, :, 0], kv[:, :, 1], lens=lens)
+    some = torch.cat([torch.arange(50), torch.arange(n - 50, n)]).cuda()
+    part = kv[some]
+    assert torch.equal(_check_cross(ops, q[some], part[:, :, 0], part[:, :, 1], lens=lens[some]), out[some])
+
+
 def test_repeated_calls_give_the_same_bits(ops):
     s = _together(ops, 40, tk=5000)
     s['elens'] = torch.tensor([5000, 4999, 3000], dtype=torch.int32).cuda()
