@@ -189,6 +189,18 @@ __device__ inline void cut(const uint32_t (&x)[8], u32x4 (&t)[3])
         t[2][j] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a2), 0x07060302u);
     }
 }
+// eight float16 values as two bf16 vectors that add up to them
+__device__ inline void cut_f16(const u32x4& x, u32x4 (&t)[2])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x2 y = unpack16<true>(x[j]);
+        const uint32_t hi = pack_bf16(y[0], y[1]);
+        const f32x2 z = unpack16<false>(hi);
+        t[0][j] = hi;
+        t[1][j] = pack_bf16(y[0] - z[0], y[1] - z[1]);
+    }
+}
 // c + a b over bf16 terms of a and b, those above 2^-24 of the product, the smallest first
 template <bool F16, int NA, int NB> __device__ inline f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c)
 {
@@ -246,15 +258,7 @@ void attention_few_kernel(AttnArgs a)
                 const uint32_t x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 cut(x, qf[t][u]);
             } else {
-                const u32x4 w = in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x2 y = unpack16<true>(w[j]);
-                    const uint32_t hi = pack_bf16(y[0], y[1]);
-                    const f32x2 z = unpack16<false>(hi);
-                    qf[t][u][0][j] = hi;
-                    qf[t][u][1][j] = pack_bf16(y[0] - z[0], y[1] - z[1]);
-                }
+                cut_f16(in ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{}, qf[t][u]);
             }
         }
     }
@@ -529,7 +533,7 @@ void attention_few_kernel(AttnArgs a)
 }
 
 // ---- many rows: the waves of a workgroup share tiles of keys in LDS ------------------------------------------------------
-// 16-bit products only.  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
+// 16-bit products only (codes with a float16 q: q and the probabilities as two bf16 terms each, which keep float16's bits).  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
 // (K three buffers, V two: the next tiles' loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
 // scale).  32 x 32 x 16 products: S^T = K q^T has a row in each lane of 32 and lane half; O^T = V^T P^T takes V^T from LDS with the transposing read
 // (four keys of one column a lane) and P^T straight from the accumulators, rounded once to the products' type.
@@ -583,6 +587,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 {
     constexpr bool F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
     constexpr bool DIRECT = FULL && !CODES;
+    constexpr int TERMS = CODES && QT == ASR_F16 ? 2 : 1;                          // bf16 terms of a value of q and of a probability
     constexpr int PITCH = DP * 2, PAIR = 128 / DP;
     constexpr int ROW_LOADS = DP / (CODES ? 16 : 8);                            // 16-byte loads of a key row
     constexpr int LOADS = MANY_KEYS * ROW_LOADS / (64 * MANY_WAVES);              // of a thread, for K and for V
@@ -606,7 +611,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 
     // q as second operand (a negative factor is moved into it: exact)
     const float c = fmaxf(fabsf(a.c), 1e-37f);                                        // (a factor of 0 must leave -infinity what it is)
-    u32x4 qf[NR][DP / 16];
+    u32x4 qf[NR][DP / 16][TERMS];
     int lim[NR];                                                                      // this lane's rows see keys below it
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
@@ -615,8 +620,10 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 #pragma unroll
         for (int u = 0; u < DP / 16; ++u) {
             const int at = 16 * u + 8 * half;
-            qf[t][u] = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
-            if (a.c < 0) qf[t][u] ^= 0x80008000u;
+            u32x4 w = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
+            if (a.c < 0) w ^= 0x80008000u;
+            if constexpr (TERMS == 2) cut_f16(w, qf[t][u]);
+            else qf[t][u][0] = w;
         }
         lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
     }
@@ -757,7 +764,9 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         return *(const __attribute__((address_space(3))) u32x4*)(kf_at[u] + 32 * sub * PITCH);
     };
     const auto score = [&](const u32x4& k, int r, int u, f32x16& s) __attribute__((always_inline)) {
-        s = mfma32<F16>(k, qf[r][u], u == 0 ? f32x16{} : s);
+        if (u == 0) s = f32x16{};
+#pragma unroll
+        for (int term = TERMS - 1; term >= 0; --term) s = mfma32<F16>(k, qf[r][u][term], s);
     };
     const auto most = [&](const f32x16& s) __attribute__((always_inline)) {
         float x = s[0];
@@ -820,7 +829,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         constexpr int SLOTS = N * NR, VALUES = 16 * NR, FROM = SLOTS / 4 < 2 ? 1 : SLOTS / 2 - 2 < 2 ? SLOTS / 2 - 2 : 2;
         u32x4 vf[N];
         float x[NR][16], most_of[NR][2];
-        uint32_t pf[NR][8];
+        uint32_t pf[TERMS][NR][8];
         // value e in the order in which they are needed: the first 16 keys' of every row tile, then the others'
         const auto row_of = [](int e) { return e / 8 % NR; };
         const auto key_of = [](int e) { return 8 * (e / (8 * NR)) + e % 8; };
@@ -836,8 +845,15 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 #pragma unroll
             for (int i = taken(w - 2) / 2; i < taken(w - 1) / 2; ++i) {
                 const int r = row_of(2 * i), j = key_of(2 * i);
-                pf[r][j / 2] = pack16<F16>(x[r][j], x[r][j + 1]);
-                l[r] = pair_sum<F16>(pf[r][j / 2], l[r]);
+                const uint32_t w = pack16<F16>(x[r][j], x[r][j + 1]);
+                pf[0][r][j / 2] = w;
+                l[r] = pair_sum<F16>(w, l[r]);
+                if constexpr (TERMS == 2) {
+                    const f32x2 y = unpack16<F16>(w);
+                    const uint32_t rest = pack16<F16>(x[r][j] - y[0], x[r][j + 1] - y[1]);
+                    pf[1][r][j / 2] = rest;
+                    l[r] = pair_sum<F16>(rest, l[r]);
+                }
             }
         };
 #pragma unroll
@@ -863,7 +879,11 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
                 if (q + AHEAD < N) vf[q + AHEAD] = v_frag(q + AHEAD);
                 else kf[q + AHEAD - N] = k_frag(buf_after, sub, q + AHEAD - N);
             }
-            o[r][i] = mfma32<F16>(vf[q], u32x4{pf[r][4 * k16], pf[r][4 * k16 + 1], pf[r][4 * k16 + 2], pf[r][4 * k16 + 3]}, o[r][i]);
+#pragma unroll
+            for (int term = TERMS - 1; term >= 0; --term) {
+                const uint32_t* x = pf[term][r] + 4 * k16;
+                o[r][i] = mfma32<F16>(vf[q], u32x4{x[0], x[1], x[2], x[3]}, o[r][i]);
+            }
             bring(SLOTS + w);
             __builtin_amdgcn_sched_barrier(0);
             between(SLOTS + w);
@@ -1074,18 +1094,20 @@ struct Plan {
     int64_t ws_bytes;
 };
 
-// sixteen: 16-bit products of one term each (bf16 or f16 keys, or codes with a bf16 query)
-Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, bool sixteen)
+// terms: 16-bit terms of a value of q (and of a probability of many rows); 3: float32
+Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, int terms)
 {
     Plan p{};
     p.rows = (int)(tq * (heads / kv_heads));
-    p.many = sixteen && p.rows > 40;            // (48 rows of 64 over 1000 states: 51 us and 55 with the other, 40 rows: 23 and 20)
+    // (48 rows of 64 over 1000 states: 51 us and 55 with the other, 40 rows: 23 and 20; with two terms 96 rows of 128 over 4096 tokens: 31 and 35, of 64 over
+    // 1024: 28 and 25.5, 64 rows: 29 and 25)
+    p.many = terms < 3 && p.rows > (terms == 1 ? 40 : 80);
     if (p.many) {
         // two row tiles a wave where its registers hold them and workgroups of twice the rows still give every compute unit two, without many idle rows (8 x 512
         // queries of 32 heads over 4096 states of 8 heads of 64: 174 us with one, 156 with two, half of them 92 and 88; heads of 128 would leave one wave a SIMD: 152
         // and 160)
         const int64_t tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
-        p.nq = d == 64 && (tiles % 2 == 0 || tiles >= 8) && n * kv_heads * ((tiles + 1) / 2) >= 512 ? 2 : 1;
+        p.nq = terms == 1 && d == 64 && (tiles % 2 == 0 || tiles >= 8) && n * kv_heads * ((tiles + 1) / 2) >= 512 ? 2 : 1;
         p.tiles = (int)((tiles + p.nq - 1) / p.nq);
         const int64_t wgs = n * kv_heads * p.tiles, most = tk / (MANY_KEYS * 8);
         int64_t split = wgs > 0 ? 512 / wgs : 1;
@@ -1120,7 +1142,9 @@ template <int QT, int KVT> hipError_t launch_few(const AttnArgs& a, int nq, hipS
 template <int QT, int KVT> hipError_t launch_many(const AttnArgs& a, int nr, hipStream_t s)
 {
     const dim3 grid((uint32_t)((int64_t)a.n * a.kv_heads * a.nsplit * a.tiles)), block(64 * MANY_WAVES);
-    if (a.d == 64) return nr == 2 ? ops_launch(attention_many_kernel<QT, KVT, 64, 2, true>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 64, 1, true>, grid, block, s, a);
+    if constexpr (!(QT == ASR_F16 && KVT == KV_E4M3))
+        if (a.d == 64 && nr == 2) return ops_launch(attention_many_kernel<QT, KVT, 64, 2, true>, grid, block, s, a);
+    if (a.d == 64) return ops_launch(attention_many_kernel<QT, KVT, 64, 1, true>, grid, block, s, a);
     if (a.d == 128) return ops_launch(attention_many_kernel<QT, KVT, 128, 1, true>, grid, block, s, a);
     return a.d < 64 ? ops_launch(attention_many_kernel<QT, KVT, 64, 1, false>, grid, block, s, a) : ops_launch(attention_many_kernel<QT, KVT, 128, 1, false>, grid, block, s, a);
 }
@@ -1143,7 +1167,7 @@ template <int QT, int KVT> int attend(const char* what, AttnArgs& a, const Plan&
         a.ws = static_cast<float*>(ws);
     }
     hipError_t e;
-    if constexpr (QT != ASR_F32 && !(QT == ASR_F16 && KVT == KV_E4M3)) e = p.many ? launch_many<QT, KVT>(a, p.nq, s) : launch_few<QT, KVT>(a, p.nq, s);
+    if constexpr (QT != ASR_F32) e = p.many ? launch_many<QT, KVT>(a, p.nq, s) : launch_few<QT, KVT>(a, p.nq, s);
     else e = launch_few<QT, KVT>(a, p.nq, s);
     if (e == hipSuccess && p.nsplit > 1) e = launch_join<QT>(a, s);
     return ops_launched(what, e);
@@ -1171,7 +1195,7 @@ extern "C" {
 int64_t asr_cross_attention_workspace(int32_t n, int32_t tq, int32_t tk, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype)
 {
     if (bad_sizes(n, tq, tk, heads, kv_heads, d, 8) || !ops_dtype_ok(dtype)) return 0;
-    return plan_of(n, tq, tk, heads, kv_heads, d, dtype != ASR_F32).ws_bytes;
+    return plan_of(n, tq, tk, heads, kv_heads, d, dtype == ASR_F32 ? 3 : 1).ws_bytes;
 }
 
 int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
@@ -1199,7 +1223,7 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
     }
     x.n = a->n; x.tq = a->tq; x.tk = a->tk; x.kv_heads = a->kv_heads; x.group = a->heads / a->kv_heads; x.d = a->d;
     x.c = a->scale * LOG2E;
-    const Plan p = plan_of(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d, a->dtype != ASR_F32);
+    const Plan p = plan_of(a->n, a->tq, a->tk, a->heads, a->kv_heads, a->d, a->dtype == ASR_F32 ? 3 : 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->dtype == ASR_F32) return attend<ASR_F32, KV_F32>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
     if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_BF16>("cross_attention", x, p, a->workspace, a->workspace_bytes, s);
@@ -1209,7 +1233,7 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream)
 int64_t asr_kv8_attention_workspace(int32_t n, int32_t tq, int32_t capacity, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype)
 {
     if (bad_sizes(n, tq, capacity, heads, kv_heads, d, 16) || !ops_dtype_ok(dtype)) return 0;
-    return plan_of(n, tq, capacity, heads, kv_heads, d, dtype == ASR_BF16).ws_bytes;
+    return plan_of(n, tq, capacity, heads, kv_heads, d, dtype == ASR_F32 ? 3 : dtype == ASR_F16 ? 2 : 1).ws_bytes;
 }
 
 int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
@@ -1241,7 +1265,7 @@ int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
     x.n = a->n; x.tq = a->tq; x.tk = a->capacity; x.kv_heads = a->kv_heads; x.group = a->heads / a->kv_heads; x.d = a->d;
     x.causal = a->causal ? 1 : 0;
     x.c = a->scale * LOG2E;
-    const Plan p = plan_of(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d, a->dtype == ASR_BF16);
+    const Plan p = plan_of(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d, a->dtype == ASR_F32 ? 3 : a->dtype == ASR_F16 ? 2 : 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->dtype == ASR_F32) return attend<ASR_F32, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
     if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);

@@ -366,7 +366,7 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream);
 /* asr_cross_attention with the cache above for keys and values; lens[b] tokens are valid (taken as 0 below 0, as the capacity above it).
  * causal: query i of sequence b is its token lens[b] - tq + i and sees nothing behind itself (the cache already holds the tq newest tokens; a
  * query with nothing to see gives 0; NaN in later tokens does not reach it).  Codes are multiplied exactly on the 16-bit matrix instruction; a q of f16 or f32 enters as
- * two or three bf16 terms, so nothing of it is lost. */
+ * two or three bf16 terms, so nothing of it is lost; probabilities as two or three (with bf16 and more than 40 rows as one). */
 typedef struct asr_kv8_attention_args {
     const void* q;
     void* out;
