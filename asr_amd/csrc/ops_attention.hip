@@ -1109,7 +1109,9 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
         const int64_t tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
         p.nq = terms == 1 && d == 64 && (tiles % 2 == 0 || tiles >= 8) && n * kv_heads * ((tiles + 1) / 2) >= 512 ? 2 : 1;
         p.tiles = (int)((tiles + p.nq - 1) / p.nq);
-        const int64_t wgs = n * kv_heads * p.tiles, most = tk / (MANY_KEYS * 8);
+        // shares of at least eight tiles, with few workgroups of four where there are twelve (joining them is a launch: 4 x 61 queries of 16 heads over 1000 states,
+        // 64 workgroups, 24.7 us in one share and 18.4 in three; 8 x 61 over 800, 128 workgroups, 16.8 and 19.9; 2 x 100 over 1500, 32 workgroups, 19.5 and 15.5)
+        const int64_t wgs = n * kv_heads * p.tiles, most = wgs <= 64 && tk >= 12 * MANY_KEYS ? tk / (MANY_KEYS * 4) : tk / (MANY_KEYS * 8);
         int64_t split = wgs > 0 ? 512 / wgs : 1;
         if (split > most) split = most;
         if (split > 16) split = 16;
