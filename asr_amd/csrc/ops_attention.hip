@@ -1122,8 +1122,9 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
     p.nq = p.rows > 16 ? 2 : 1;
     p.tiles = (p.rows + 16 * p.nq - 1) / (16 * p.nq);
     // shares of the key axis: enough workgroups for the chip (three for each of 256 compute units: 16 x 4 queries over 4096 f32 keys 41 us with one, 31 with
-    // two, 29 with three), each with at least four chunks of 32 keys for each wave
-    const int64_t wgs = n * kv_heads * p.tiles, most = tk / (FEW_WAVES * 32 * 4);
+    // two, 29 with three), each with at least four chunks of 32 keys for each wave, or two where a few workgroups have a short axis (one token over 1000 f32 states,
+    // 16 workgroups: 17 us and 12.2 with two; 14 x 25 over 832 bf16 tokens, 70: 12.9 and 11.6; but 8 x 10 over 600, 128: 8.5 and 10.2; 7 x 29 x 8 over 4587: 28.7 and 34)
+    const int64_t wgs = n * kv_heads * p.tiles, most = tk / (FEW_WAVES * 32 * (wgs <= 80 && tk <= 2048 ? 2 : 4));
     int64_t split = wgs > 0 ? (768 + wgs - 1) / wgs : 1;
     if (split > most) split = most;
     if (split > 64) split = 64;
