@@ -346,8 +346,9 @@ template <int DT> hipError_t run_token_logprobs(const TokenLogprobsArgs& k, hipS
     if (k.rows <= 256 && k.vocab / Elem<DT>::PER >= 2048) return ops_launch(token_logprobs_kernel<DT, 1024>, grid, dim3(1024), s, k);
     // Short rows: one wave has a few loads for each thread and meets nobody, and its 64 strips are the groups of the bound - spread over 256 threads they fill so
     // few groups that most of the row becomes candidates (2991 x 197 f32, top 13: 36 us with 256 threads, 7.3 with 64; 3000 x 2000 bf16, top 10: 13.4 and 9;
-    // 100 x 1000 bf16, top 32: 56 and 8.7; 10 x 1000 f32: 5.5 and 5.4)
-    if (k.vocab / Elem<DT>::PER <= 256) return ops_launch(token_logprobs_kernel<DT, 64>, grid, dim3(64), s, k);
+    // 100 x 1000 bf16, top 32: 56 and 8.7; 10 x 1000 f32: 5.5 and 5.4).  Longer ones too where there are
+    // rows enough for every wave (20000 x 3000 bf16: 62 and 32; 3000 x 7000: 16.4 and 14.7; but 200 x 4000: 6.4 and 7.7)
+    if (k.vocab / Elem<DT>::PER <= (k.rows >= 1024 ? 1024 : 256)) return ops_launch(token_logprobs_kernel<DT, 64>, grid, dim3(64), s, k);
     return ops_launch(token_logprobs_kernel<DT, 256>, grid, dim3(256), s, k);
 }
 
