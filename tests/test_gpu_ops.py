@@ -110,6 +110,19 @@ def test_token_logprobs_masks_and_extremes(ops, dtype, vocab):
     _check_logprobs(ops, x.cuda(), torch.zeros_like(tokens).cuda(), 32)
 
 
+@pytest.mark.parametrize('dtype,vocab', [('f32', 2003), ('bf16', 5003), ('f16', 8191)])
+def test_token_logprobs_of_many_longer_rows(ops, dtype, vocab):
+    """A thousand rows: ordinary ones, a third masked, equal logits throughout, all masked but a few, all masked."""
+    g = _gen(vocab)
+    x = torch.randn(1030, vocab, generator=g) * 3
+    x[200:400].masked_fill_(torch.rand(200, vocab, generator=g) < 1 / 3, -math.inf)
+    x[400:410] = 1.5
+    x[410:420] = -math.inf
+    x[410:415, 7:13] = torch.randn(5, 6, generator=g)
+    tokens = torch.randint(-1, vocab, (1030,), generator=g)
+    _check_logprobs(ops, x.to(TYPES[dtype]).cuda(), tokens.cuda(), 9)
+
+
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
 def test_token_logprobs_tokens_outside_the_vocabulary(ops, dtype):
     g = _gen(9)
