@@ -533,15 +533,16 @@ void attention_few_kernel(AttnArgs a)
 }
 
 // ---- many rows: the waves of a workgroup share tiles of keys in LDS ------------------------------------------------------
-// 16-bit products only (codes with a float16 q: q and the probabilities as two bf16 terms each, which keep float16's bits).  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
+// 16-bit products only, the probabilities as two terms like those of few rows (codes with a float16 q: q as two bf16 terms too, which keep its bits).  One term would
+// save a third of the products and round every probability to 8 bits: as much error as the result's own rounding adds (8 x 768 queries of 32 heads over 4001 states of 8
+// heads of 128: 440 us and 0.0017 of the result with two, 322 us and 0.0023 with one).  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
 // (K three buffers, V two: the next tiles' loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
 // scale).  32 x 32 x 16 products: S^T = K q^T has a row in each lane of 32 and lane half; O^T = V^T P^T takes V^T from LDS with the transposing read
-// (four keys of one column a lane) and P^T straight from the accumulators, rounded once to the products' type.
+// (four keys of one column a lane) and P^T straight from the accumulators: what a term lacks is exact in float32 and becomes the next one.
 // The 16-byte chunks of a row are permuted by its number (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4), by pairs of rows where rows are half
 // as long): both kinds of read then meet every bank evenly.  Rows of 16-bit values as long as the tile go from memory to LDS directly.
-// What bounds it: instructions.  A tile is 32 products (1024 cycles of the matrix pipe) and some 190 vector instructions a wave and row tile; products of one
-// wave run beside the vector instructions of both waves of a SIMD, but a wave alone issues only every 7 cycles.  8 x 768 queries of 32 heads over 4001
-// states of 8 heads of 128: 1000 TFLOP/s while all workgroups run.
+// What bounds it: instructions.  A tile is 48 products (1536 cycles of the matrix pipe) and some 290 vector instructions a wave and row tile; products of one
+// wave run beside the vector instructions of both waves of a SIMD, but a wave alone issues only every 7 cycles.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;               // (MANY_ROWS: for each row tile of a wave)
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -587,7 +588,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 {
     constexpr bool F16 = KVT == KV_F16, CODES = KVT == KV_E4M3;
     constexpr bool DIRECT = FULL && !CODES;
-    constexpr int TERMS = CODES && QT == ASR_F16 ? 2 : 1;                          // bf16 terms of a value of q and of a probability
+    constexpr int QTERMS = CODES && QT == ASR_F16 ? 2 : 1, PTERMS = 2;             // 16-bit terms of a value of q, of a probability
     constexpr int PITCH = DP * 2, PAIR = 128 / DP;
     constexpr int ROW_LOADS = DP / (CODES ? 16 : 8);                            // 16-byte loads of a key row
     constexpr int LOADS = MANY_KEYS * ROW_LOADS / (64 * MANY_WAVES);              // of a thread, for K and for V
@@ -611,7 +612,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 
     // q as second operand (a negative factor is moved into it: exact)
     const float c = fmaxf(fabsf(a.c), 1e-37f);                                        // (a factor of 0 must leave -infinity what it is)
-    u32x4 qf[NR][DP / 16][TERMS];
+    u32x4 qf[NR][DP / 16][QTERMS];
     int lim[NR];                                                                      // this lane's rows see keys below it
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
@@ -622,7 +623,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
             const int at = 16 * u + 8 * half;
             u32x4 w = at < a.d && r < a.rows ? *reinterpret_cast<const u32x4*>(qp + 2 * at) : u32x4{};
             if (a.c < 0) w ^= 0x80008000u;
-            if constexpr (TERMS == 2) cut_f16(w, qf[t][u]);
+            if constexpr (QTERMS == 2) cut_f16(w, qf[t][u]);
             else qf[t][u][0] = w;
         }
         lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
@@ -766,7 +767,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
     const auto score = [&](const u32x4& k, int r, int u, f32x16& s) __attribute__((always_inline)) {
         if (u == 0) s = f32x16{};
 #pragma unroll
-        for (int term = TERMS - 1; term >= 0; --term) s = mfma32<F16>(k, qf[r][u][term], s);
+        for (int term = QTERMS - 1; term >= 0; --term) s = mfma32<F16>(k, qf[r][u][term], s);
     };
     const auto most = [&](const f32x16& s) __attribute__((always_inline)) {
         float x = s[0];
@@ -829,7 +830,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         constexpr int SLOTS = N * NR, VALUES = 16 * NR, FROM = SLOTS / 4 < 2 ? 1 : SLOTS / 2 - 2 < 2 ? SLOTS / 2 - 2 : 2;
         u32x4 vf[N];
         float x[NR][16], most_of[NR][2];
-        uint32_t pf[TERMS][NR][8];
+        uint32_t pf[PTERMS][NR][8];
         // value e in the order in which they are needed: the first 16 keys' of every row tile, then the others'
         const auto row_of = [](int e) { return e / 8 % NR; };
         const auto key_of = [](int e) { return 8 * (e / (8 * NR)) + e % 8; };
@@ -846,14 +847,11 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
             for (int i = taken(w - 2) / 2; i < taken(w - 1) / 2; ++i) {
                 const int r = row_of(2 * i), j = key_of(2 * i);
                 const uint32_t w = pack16<F16>(x[r][j], x[r][j + 1]);
+                const f32x2 y = unpack16<F16>(w);
+                const uint32_t rest = pack16<F16>(x[r][j] - y[0], x[r][j + 1] - y[1]);
                 pf[0][r][j / 2] = w;
-                l[r] = pair_sum<F16>(w, l[r]);
-                if constexpr (TERMS == 2) {
-                    const f32x2 y = unpack16<F16>(w);
-                    const uint32_t rest = pack16<F16>(x[r][j] - y[0], x[r][j + 1] - y[1]);
-                    pf[1][r][j / 2] = rest;
-                    l[r] = pair_sum<F16>(rest, l[r]);
-                }
+                pf[1][r][j / 2] = rest;
+                l[r] = pair_sum<F16>(rest, pair_sum<F16>(w, l[r]));
             }
         };
 #pragma unroll
@@ -880,7 +878,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
                 else kf[q + AHEAD - N] = k_frag(buf_after, sub, q + AHEAD - N);
             }
 #pragma unroll
-            for (int term = TERMS - 1; term >= 0; --term) {
+            for (int term = PTERMS - 1; term >= 0; --term) {
                 const uint32_t* x = pf[term][r] + 4 * k16;
                 o[r][i] = mfma32<F16>(vf[q], u32x4{x[0], x[1], x[2], x[3]}, o[r][i]);
             }
@@ -1094,18 +1092,19 @@ struct Plan {
     int64_t ws_bytes;
 };
 
-// terms: 16-bit terms of a value of q (and of a probability of many rows); 3: float32
+// terms: 16-bit terms of a value of q; 3: float32
 Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads, int64_t d, int terms)
 {
     Plan p{};
     p.rows = (int)(tq * (heads / kv_heads));
-    // (48 rows of 64 over 1000 states: 51 us and 55 with the other, 40 rows: 23 and 20; with two terms 96 rows of 128 over 4096 tokens: 31 and 35, of 64 over
-    // 1024: 28 and 25.5, 64 rows: 29 and 25)
-    p.many = terms < 3 && p.rows > (terms == 1 ? 40 : 80);
+    // us of few rows and of many: 50 x 16 heads of 64 over 1000 states, 64 rows: 50.7 and 56, 80: 67 and 58; 8 x 16 of them, 64: 14.4 and 22, 128: 18 and 23; 16 x 8 heads of 128
+    // over 2000, 33: 40 and 36, 64: 42 and 39, 80: 52 and 41; 2 x 8 of them over 4096, 64: 15.8 and 18.5, 96: 21.4 and 20.4; over codes 8 x 8 heads of 128 and 4096 tokens, 64: 33 and
+    // 33, 80: 40 and 35; 32 x 16 of 64 and 1024, 64: 23 and 32, 80: 32 and 32; the same with float16 queries, 64: 30 and 35, 80: 37 and 33
+    p.many = terms < 3 && p.rows > 64;
     if (p.many) {
         // two row tiles a wave where its registers hold them and workgroups of twice the rows still give every compute unit two, without many idle rows (8 x 512
-        // queries of 32 heads over 4096 states of 8 heads of 64: 174 us with one, 156 with two, half of them 92 and 88; heads of 128 would leave one wave a SIMD: 152
-        // and 160)
+        // queries of 32 heads over 4096 states of 8 heads of 64: 230 us with one, 220 with two, though those spill some twenty registers; heads of 128 would leave one
+        // wave a SIMD)
         const int64_t tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
         p.nq = terms == 1 && d == 64 && (tiles % 2 == 0 || tiles >= 8) && n * kv_heads * ((tiles + 1) / 2) >= 512 ? 2 : 1;
         p.tiles = (int)((tiles + p.nq - 1) / p.nq);

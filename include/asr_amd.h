@@ -320,8 +320,8 @@ int asr_token_logprobs(const asr_token_logprobs_args* a, void* stream);
  * of one utterance are query rows (tq = beams): nothing orders the queries.
  * q, out: [n, tq, heads, d], k, v: [n, tk, kv_heads, d] of one type, d contiguous, every other stride free but such that each row starts on
  * 16 bytes; out may not overlap the inputs.  bf16 and f16 are multiplied as they are; f32 is cut into three bf16 terms (exact) of whose nine products the six
- * above 2^-24 are taken, so an infinity in an admitted f32 position gives NaN; scores, soft-max statistics and sums are float32.  With bf16 and f16 and more
- * than 40 rows (tq * heads / kv_heads) the probabilities are rounded once to that type.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
+ * above 2^-24 are taken, so an infinity in an admitted f32 position gives NaN; scores, soft-max statistics and sums are float32.  With bf16 and f16
+ * the probabilities enter as two terms of that type (2^-17 or 2^-22 of each is lost), whatever the number of rows.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
 typedef struct asr_cross_attention_args {
     const void *q, *k, *v;
     void* out;
@@ -366,7 +366,7 @@ int asr_kv8_append(const asr_kv8_append_args* a, void* stream);
 /* asr_cross_attention with the cache above for keys and values; lens[b] tokens are valid (taken as 0 below 0, as the capacity above it).
  * causal: query i of sequence b is its token lens[b] - tq + i and sees nothing behind itself (the cache already holds the tq newest tokens; a
  * query with nothing to see gives 0; NaN in later tokens does not reach it).  Codes are multiplied exactly on the 16-bit matrix instruction; a q of f16 or f32 enters as
- * two or three bf16 terms, so nothing of it is lost; probabilities as two or three (with bf16 and more than 40 rows as one). */
+ * two or three bf16 terms, so nothing of it is lost; probabilities as two, or three with f32. */
 typedef struct asr_kv8_attention_args {
     const void* q;
     void* out;

@@ -1,0 +1,76 @@
+"""Attention of asr_amd.ops against 64 bits within bounds that know in how many terms each path holds its probabilities: losing one of them is seen."""
+import pytest
+import torch
+
+from tests import ops_reference as R
+from tests.test_gpu_ops import TYPES, _close, _cross_case, _gen, _loud_cache
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def ops():
+    from asr_amd import ops as module
+    return module
+
+
+def _two_terms(out, weight, size, d, tk, dtype, codes):
+    """R.attention_bound without its half step of a 16-bit probability: one held as the sum of two terms, each rounded to the nearest, is off by the
+    square of a half step (bf16, and every type over codes: 2^-16; float16: 2^-22), a float32 one over three terms by nothing that counts.  What is left
+    is the scores' error, the exponential's, the sums' and the result's own rounding."""
+    p = 2 * (d + 8) * R.U * size + 2.0 ** -22 + (tk / 8 + 64) * R.U
+    if dtype != torch.float32:
+        p = p + R.HALF_STEP[torch.bfloat16 if codes else dtype] ** 2
+    return 2 * p * weight + R.HALF_STEP[dtype] * out.abs() + 1e-30
+
+
+def _check_cross(ops, q, k, v, lens, pad):
+    n, tq, _, d = q.shape
+    tk = k.shape[1]
+    admitted = (torch.arange(tk) < lens[:, None]) & ~pad
+    got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), lens=lens.cuda(), pad=pad.cuda())
+    want, weight, size = R.attention(q, k.double().transpose(1, 2), v.double().transpose(1, 2), admitted[:, None].expand(n, tq, tk), d ** -0.5)
+    _close(got, want, _two_terms(want, weight, size, d, tk, q.dtype, False), 'out')
+
+
+def _check_kv8(ops, q, cache, lens, causal):
+    n, tq, _, d = q.shape
+    tk = cache[0].shape[2]
+    got = ops.kv8_attention(q.cuda(), *cache, lens.cuda(), causal=causal)
+    k, v = (R.values_of(c) * s.cpu().double().repeat_interleave(64, -1)[..., None] for c, s in (cache[::2], cache[1::2]))
+    last = lens.long()[:, None].expand(n, tq)
+    if causal:
+        last = last - tq + 1 + torch.arange(tq)
+    want, weight, size = R.attention(q, k, v, torch.arange(tk) < last[..., None], d ** -0.5)
+    _close(got, want, _two_terms(want, weight, size, d, tk, q.dtype, True), 'out')
+
+
+CROSS = [(2, 1, 47, 2, 2, 64), (2, 10, 334, 4, 2, 64), (1, 40, 300, 2, 2, 128), (1, 41, 300, 2, 2, 128), (2, 61, 300, 4, 2, 64), (2, 64, 300, 2, 2, 64), (2, 65, 300, 2, 2, 64), (1, 200, 1100, 2, 1, 80),
+         (1, 4, 4000, 2, 1, 64), (64, 256, 70, 8, 8, 64)]
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('shape', CROSS, ids=str)
+def test_cross_attention_holds_two_terms_of_a_probability(ops, shape, dtype):
+    n, _, tk = shape[:3]
+    if dtype == 'f32' and n == 64:
+        n, shape = 4, (4,) + shape[1:]                      # (float32 has no kernel of its own for many rows)
+    q, kv = _cross_case(sum(shape) + 1, *shape, dtype)
+    lens = torch.randint((tk + 1) // 2, tk + 1, (n,), generator=_gen(tk), dtype=torch.int32)
+    pad = torch.rand(n, tk, generator=_gen(n)) < 0.1
+    _check_cross(ops, q, kv[:, :, 0], kv[:, :, 1], lens, pad)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('n,tq,heads,kv_heads,capacity,d', [(2, 1, 4, 2, 192, 64), (2, 10, 4, 2, 320, 128), (2, 20, 4, 2, 320, 64), (2, 21, 4, 2, 320, 64), (2, 33, 4, 2, 320, 64),
+                                                            (2, 100, 4, 2, 320, 128), (1, 300, 2, 2, 1088, 80), (1, 2, 8, 1, 4096, 128),
+                                                            (64, 128, 16, 8, 192, 64)])
+def test_kv8_attention_holds_two_terms_of_a_probability(ops, n, tq, heads, kv_heads, capacity, d, causal, dtype):
+    g = _gen(n + tq + capacity)
+    if dtype != 'bf16' and n == 64:
+        n = 4
+    cache = _loud_cache(ops, g, n, kv_heads, capacity, d)
+    q = torch.randn(n, tq, heads, d, generator=g).to(TYPES[dtype])
+    lens = torch.randint(max(tq, capacity // 2), capacity + 1, (n,), generator=g, dtype=torch.int32)
+    _check_kv8(ops, q, cache, lens, causal)
