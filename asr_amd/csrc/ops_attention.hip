@@ -111,9 +111,10 @@ __device__ inline float groups_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// m follows a row's maximum (in powers of two) only when that grows by more than SLACK: P is at most 2^SLACK then, its rounding is relative as before, and
-// nearly all tiles skip the scaling of the sums.  It starts finite, so that no difference with it is NaN.
-constexpr float SLACK = 8.0f, NO_MAX = -3.0e38f;
+// P = 2^(score - m).  m follows a row's maximum (in powers of two) only when that grows by more than SLACK: P is at most 2^SLACK then, its rounding is relative as before, and
+// nearly all tiles skip the scaling of the sums.  It starts finite, so that no difference with it is NaN.  A float16 P is relative down to 2^-14 and 0 below 2^-25: there m stays
+// LIFT below the maximum that it follows, so that the largest P of a row is 2^7 to 2^15 and keys 22 nats below it still count (a largest one of 1 lost those 17 nats below).
+constexpr float SLACK = 8.0f, LIFT16 = 7.0f, NO_MAX = -3.0e38f;
 __device__ inline float rescale(float m_old, float m_new) { return __builtin_amdgcn_exp2f(m_old - m_new); }
 
 __device__ inline int keys_of(const AttnArgs& a, int b) { return a.lens ? min(max(a.lens[b], 0), a.tk) : a.tk; }
@@ -156,7 +157,7 @@ __device__ inline int longest_first(const AttnArgs& a, int at)
 // keys are loaded as soon as the scores have been taken from this one's, the next values behind the output.  K and V are read once by each row
 // tile: bound by those bytes while there are few rows.  QT: type of q and out, KVT: of K and V.
 // Terms: 16-bit K / V are exact factors; q enters as QTERMS 16-bit terms (bf16 codes: f16 = 2, f32 = 3 bf16 terms lose nothing) and
-// P as PTERMS (two: 2^-17 / 2^-22 of it lost, three: nothing), which costs matrix instructions that a loop waiting for memory has to spare.
+// P as PTERMS (two: 2^-17 of it lost, of float16 2^-22 or 2^-32 of the row's largest, whichever is more; three: nothing), which costs matrix instructions that a loop waiting for memory has to spare.
 // float32 K / V are cut into three bf16 terms as well (8 + 8 + 8 bits: exact), and of the nine products the six above 2^-24 are taken: the 16-bit matrix
 // pipe is 16 times the float32 one, which besides shares its units with the vector instructions (50 x 61 queries over 1000 states of 16 heads:
 // 133 us on the float32 instruction, 108 so).
@@ -336,6 +337,7 @@ void attention_few_kernel(AttnArgs a)
         }
     };
 
+    constexpr float LIFT = F::F16 ? LIFT16 : 0.0f;
     uint64_t nan_seen = 0;
     int chunk = chunk0 + wave;
     if (chunk < chunk1) {
@@ -391,8 +393,8 @@ void attention_few_kernel(AttnArgs a)
 #pragma unroll
             for (int j = 1; j < 8; ++j) top = fmaxf(top, p[t][j]);
             top = groups_max(top);
-            if (__ballot(top > m[t] + SLACK)) {
-                const float grown = fmaxf(m[t], top), f = rescale(m[t], grown);
+            if (__ballot(top - m[t] > SLACK + LIFT)) {                         // (the difference: exact where m + SLACK would be rounded)
+                const float grown = fmaxf(m[t], top - LIFT), f = rescale(m[t], grown);
                 m[t] = grown;
                 l[t] *= f;
 #pragma unroll
@@ -773,12 +775,14 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         float x = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) x = fmaxf(x, s[i]);
-        return halves_max(x) * c;
+        return halves_max(x);
     };
     uint64_t grow = 0;                                                               // the lanes whose rows' maximum has grown
+    constexpr float LIFT = F16 ? LIFT16 : 0.0f;
+    const auto grown_by = [&](int r) __attribute__((always_inline)) { return fmaf(top[r], c, -m[r]); };         // (what the exponentials take: none is above it)
     const auto grows = [&]() __attribute__((always_inline)) {
-        bool x = top[0] > m[0] + SLACK;
-        if (NR > 1) x |= top[NR - 1] > m[NR - 1] + SLACK;
+        bool x = grown_by(0) > SLACK + LIFT;
+        if (NR > 1) x |= grown_by(NR - 1) > SLACK + LIFT;
         return __ballot(x);
     };
     // soft-max and output of half `sub` of tile t from its scores s with their maxima `top`, and the scores of the half behind it.  The products are laid out
@@ -808,7 +812,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         if (grow) {
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                const float grown = top[r] > m[r] + SLACK ? top[r] : m[r], f = rescale(m[r], grown);
+                const float grown = grown_by(r) > SLACK + LIFT ? top[r] * c - LIFT : m[r], f = rescale(m[r], grown);
                 m[r] = grown;
                 l[r] *= f;
 #pragma unroll
@@ -902,7 +906,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
             if (w == FROM + SLOTS / 2) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    top[r] = halves_max(fmaxf(most_of[r][0], most_of[r][1])) * c;
+                    top[r] = halves_max(fmaxf(most_of[r][0], most_of[r][1]));
                     asm volatile("" : "+v"(top[r]));
                 }
             }

@@ -74,3 +74,54 @@ def test_kv8_attention_holds_two_terms_of_a_probability(ops, n, tq, heads, kv_he
     q = torch.randn(n, tq, heads, d, generator=g).to(TYPES[dtype])
     lens = torch.randint(max(tq, capacity // 2), capacity + 1, (n,), generator=g, dtype=torch.int32)
     _check_kv8(ops, q, cache, lens, causal)
+
+
+# ---- float16: the soft-max's tail --------------------------------------------------------------------------------------------
+def _tail_bound(out, weight, size, d, tk, vmax):
+    """_two_terms for float16 K and V, whose terms have a smallest step of 2^-24: the largest probability of a row enters as at least 2^7, so each is off by
+    at most 2^-25 / 2^7 = 2^-32 of it besides what is relative, in the sum over V and, where the row sum has the unrounded ones, once more in the weights."""
+    return _two_terms(out, weight, size, d, tk, torch.float16, False) + 2 * tk * 2.0 ** -32 * vmax
+
+
+@pytest.mark.parametrize('nats', [10.0, 14.0, 15.0, 16.0, 17.5, 19.0])
+@pytest.mark.parametrize('tq,tk,d', [(1, 4097, 64), (16, 300, 64), (40, 4097, 128), (70, 4097, 64), (200, 1000, 128), (130, 900, 80)])
+def test_float16_attention_keeps_far_keys(ops, tq, tk, d, nats):
+    """One key far above thousands of others with a V of its own: their share is small, but not lost (1.0e-4 of 4096 keys at 17.5 nats)."""
+    q = torch.zeros(1, tq, 1, d)
+    q[..., 0] = 0.5
+    k = torch.zeros(1, tk, 1, d)
+    k[0, 1:, 0, 0] = -nats / 4                               # (times 0.5, times a scale of 8: exact)
+    k[0, :, 0, 1:] = torch.randn(tk, d - 1, generator=_gen(tk))
+    v = torch.zeros(1, tk, 1, d)
+    v[0, 1:, 0] = 1024 + 256 * torch.randint(0, 3, (tk - 1, d), generator=_gen(d))         # (no result below float16's normal ones)
+    q, k, v = q.half(), k.half(), v.half()
+    got = ops.cross_attention(q.cuda(), k.cuda(), v.cuda(), scale=8.0)
+    want, weight, size = R.attention(q, k.double().transpose(1, 2), v.double().transpose(1, 2), torch.ones(1, tq, tk, dtype=torch.bool), 8.0)
+    _close(got, want, _tail_bound(want, weight, size, d, tk, 1536.0), 'out')
+
+
+@pytest.mark.parametrize('shape', CROSS, ids=str)
+def test_cross_attention_of_float16_holds_two_terms_of_a_probability(ops, shape):
+    n, tq, tk, _, _, d = shape
+    q, kv = _cross_case(sum(shape) + 1, *shape, 'f16')
+    lens = torch.randint((tk + 1) // 2, tk + 1, (n,), generator=_gen(tk), dtype=torch.int32)
+    got = ops.cross_attention(q.cuda(), kv[:, :, 0].cuda(), kv[:, :, 1].cuda(), lens=lens.cuda())
+    k, v = (kv[:, :, i].double().transpose(1, 2) for i in (0, 1))
+    want, weight, size = R.attention(q, k, v, (torch.arange(tk) < lens[:, None])[:, None].expand(n, tq, tk), d ** -0.5)
+    _close(got, want, _tail_bound(want, weight, size, d, tk, float(v.abs().max())), 'out')
+
+
+def test_float16_attention_of_growing_scores(ops):
+    """Scores that grow by less and by more than the slack of the running maximum from tile to tile: probabilities stay finite."""
+    tk, d = 2000, 64
+    for step in (0.001, 0.02, 0.3):
+        q = torch.zeros(1, 70, 1, d)
+        q[..., 0] = 1.0
+        k = torch.zeros(1, tk, 1, d)
+        k[0, :, 0, 0] = torch.arange(tk) * step
+        v = torch.randn(1, tk, 1, d, generator=_gen(1))
+        q, k, v = q.half(), k.half(), v.half()
+        for rows in (1, 20, 70):
+            got = ops.cross_attention(q[:, :rows].cuda(), k.cuda(), v.cuda(), scale=1.0)
+            want, weight, size = R.attention(q[:, :rows], k.double().transpose(1, 2), v.double().transpose(1, 2), torch.ones(1, rows, tk, dtype=torch.bool), 1.0)
+            _close(got, want, _tail_bound(want, weight, size, d, tk, float(v.abs().max())), 'out')
