@@ -117,6 +117,32 @@ __device__ inline float groups_sum(float x)
 constexpr float SLACK = 8.0f, LIFT16 = 7.0f, NO_MAX = -3.0e38f;
 __device__ inline float rescale(float m_old, float m_new) { return __builtin_amdgcn_exp2f(m_old - m_new); }
 
+// An infinity in an admitted V: a term of P that is 0, or of the other sign than the first, makes NaN of it, as does scaling what was summed by 0, and the cut of a float32 one.
+// Where a sum is NaN though the row's P are finite, its columns of V are looked through again (bit i for column i of what a lane has): with one sign of infinity the
+// sum is that, with both or with NaN it is NaN.
+struct Seen {
+    uint32_t up = 0, down = 0, nan = 0;
+    template <int KVT> __device__ inline void add(mem p, int bit)
+    {
+        constexpr uint32_t INF = KVT == KV_F32 ? 0x7f800000u : KVT == KV_F16 ? 0x7c00u : 0x7f80u, SIGN = KVT == KV_F32 ? 0x80000000u : 0x8000u;
+        uint32_t x;
+        if constexpr (KVT == KV_F32) x = load_as<uint32_t>(p);
+        else x = load_as<uint16_t>(p);
+        const uint32_t size = x & ~SIGN;
+        up |= (uint32_t)(x == INF) << bit;
+        down |= (uint32_t)(x == (INF | SIGN)) << bit;
+        nan |= (uint32_t)(size > INF) << bit;
+    }
+    __device__ inline float instead_of(float sum, int bit) const
+    {
+        const bool u = up >> bit & 1, d = down >> bit & 1, n = nan >> bit & 1;
+        return n || (u && d) ? __builtin_nanf("") : u ? __builtin_inff() : d ? -__builtin_inff() : sum;
+    }
+};
+// x f, but an infinite x stays what it is where f is 0
+__device__ inline float scaled(float x, float f) { return __builtin_fabsf(x) == __builtin_inff() ? x : x * f; }
+__device__ inline f32x4 scaled(const f32x4& x, float f) { return f32x4{scaled(x[0], f), scaled(x[1], f), scaled(x[2], f), scaled(x[3], f)}; }
+
 __device__ inline int keys_of(const AttnArgs& a, int b) { return a.lens ? min(max(a.lens[b], 0), a.tk) : a.tk; }
 
 // Workgroup `id` -> (sequence, K/V head), and what is left of id for its row tile and share, `per` of them for each.  Consecutive workgroups go round the
@@ -514,6 +540,20 @@ void attention_few_kernel(AttnArgs a)
             const float f = rescale(s_m[w][rr], top);
             sum += s_l[w][rr] * f;
             acc += *reinterpret_cast<const f32x4*>(&s_o[w][rr][at]) * f;
+        }
+        if constexpr (!F::CODES) {
+            const float all = acc[0] + acc[1] + acc[2] + acc[3];
+            if (all != all && sum < __builtin_inff()) {
+                Seen seen;
+                for (int key = 32 * chunk0; key < min(32 * chunk1, len); ++key) {
+                    if (pad && pad[key]) continue;
+                    const mem p = (mem)vb + (int64_t)key * a.v_stride[1] + at * F::KVB;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) seen.add<KVT>(p + i * F::KVB, i);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = seen.instead_of(acc[i], i);
+            }
         }
         if (a.nsplit > 1) {
             float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
@@ -980,6 +1020,39 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
             }
         }
         wait_for_memory();                                                              // (no load into LDS may outlive its workgroup)
+        if constexpr (!CODES) {
+            bool lost = false;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                f32x4 z{};
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) z[j & 3] = fmaf(o[r][i][j], 0.0f, z[j & 3]);
+                z[0] += z[1] + z[2] + z[3];
+                lost |= z[0] != z[0] && halves_sum(l[r]) < __builtin_inff();
+            }
+            if (__ballot(lost)) {
+                Seen seen[DP / 32];
+                for (int key = t0 * MANY_KEYS; key < min(t1 * MANY_KEYS, len); ++key) {
+                    if (pad && pad[key]) continue;
+                    const mem p = (mem)vb + (int64_t)key * a.v_stride[1];
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int at = 32 * i + 8 * (j >> 2) + 4 * half + (j & 3);
+                            if (at < a.d) seen[i].template add<KVT>(p + 2 * at, j);
+                        }
+                }
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[r][i][j] = seen[i].instead_of(o[r][i][j], j);
+            }
+        }
         if constexpr (CODES) {
             if (a.causal) {
                 uint32_t* waves = reinterpret_cast<uint32_t*>(s_k);                     // (LDS is full: two workgroups share it)
@@ -1062,7 +1135,7 @@ template <int QT, int G> __global__ __launch_bounds__(256) void attention_join_k
             const float* p = ws + s * split_stride;
             const float f = rescale(p[0], top);
             sum += p[1] * f;
-            acc += *reinterpret_cast<const f32x4*>(p + 4 + (at < a.d ? at : 0)) * f;
+            acc += scaled(*reinterpret_cast<const f32x4*>(p + 4 + (at < a.d ? at : 0)), f);
         }
         *reinterpret_cast<f32x4*>(s_acc[slot][g][lane]) = acc;
         if (lane == 0) s_sum[slot][g] = sum;

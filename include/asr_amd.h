@@ -320,7 +320,8 @@ int asr_token_logprobs(const asr_token_logprobs_args* a, void* stream);
  * of one utterance are query rows (tq = beams): nothing orders the queries.
  * q, out: [n, tq, heads, d], k, v: [n, tk, kv_heads, d] of one type, d contiguous, every other stride free but such that each row starts on
  * 16 bytes; out may not overlap the inputs.  bf16 and f16 are multiplied as they are; f32 is cut into three bf16 terms (exact) of whose nine products the six
- * above 2^-24 are taken, so an infinity in an admitted f32 position gives NaN; scores, soft-max statistics and sums are float32.  With bf16 and f16
+ * above 2^-24 are taken, so an infinity in an f32 query or admitted key gives NaN.  Infinities in admitted values are the result of their column, whatever their weight (both
+ * signs: NaN).  Scores, soft-max statistics and sums are float32.  With bf16 and f16
  * the probabilities enter as two terms of that type (2^-17 of each is lost, or 2^-22 and at most 2^-32 of the row's largest), whatever the number of rows.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
 typedef struct asr_cross_attention_args {
     const void *q, *k, *v;
