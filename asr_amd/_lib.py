@@ -108,6 +108,7 @@ def _load():
         'asr_cross_attention_workspace': (i64, [i32] * 7),
         'asr_kv8_append': (i32, [C.c_char_p, vp]),
         'asr_kv8_attention': (i32, [C.c_char_p, vp]),
+        'asr_kv8_attention_counts': (i32, [C.c_char_p, vp, vp]),
         'asr_kv8_attention_workspace': (i64, [i32] * 7),
     }
     for name, (res, args) in sig.items():

@@ -31,7 +31,7 @@ struct AttnArgs {
     const char *q, *k, *v;
     char* out;
     const float *k_scale, *v_scale;      // KV_E4M3
-    const int32_t* lens;
+    const int32_t *lens, *counts;        // counts (KV_E4M3): a sequence's own queries, its first ones; null: all tq
     const uint8_t* pad;
     float* ws;                           // nsplit > 1: per (split, sequence, K/V head, row): m, l, then O [d]
     int64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3];        // bytes; of n, t, head
@@ -163,6 +163,9 @@ __device__ inline int place_of(int nbh, int per, int64_t& id)
     return bh;
 }
 
+// the queries that sequence b has; those behind them are computed like its last one and given zeros
+template <bool CODES> __device__ inline int queries_of(const AttnArgs& a, int b) { return CODES && a.counts ? min(max(a.counts[b], 0), a.tq) : a.tq; }
+
 // The sequence that is number `at` when the longest come first (at itself where that would not matter or take too long): the last workgroups of a launch
 // are then short ones (16 x 200 queries over 1500 states of half to full length: 41.5 -> 38 us; one token over 64 caches of up to 2048: 45.7 -> 42.9).  Finding it
 // costs up to half a microsecond a workgroup, too much for few rows over short keys (64 x 10 queries over 334 states: 15.5 -> 16.4 us).
@@ -258,11 +261,12 @@ void attention_few_kernel(AttnArgs a)
     const int place = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
     const int split = (int)(id % a.nsplit), tile = (int)(id / a.nsplit);
     const int b = a.tk >= 1024 ? longest_first(a, place / a.kv_heads) : place / a.kv_heads, h = place % a.kv_heads, bh = b * a.kv_heads + h;
-    const int len = keys_of(a, b), row0 = tile * 16 * NQ;
+    const int len = keys_of(a, b), row0 = tile * 16 * NQ, tq = queries_of<F::CODES>(a, b);
 
-    // this tile's keys: all of them, or in a causal call what its last row sees
+    // this tile's keys: all of them, or in a causal call what its last row sees; none without queries
     int last_key = len;
-    if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + 16 * NQ - 1, a.rows - 1) / a.group + 1));
+    if (a.causal) last_key = min(len, max(0, len - tq + min(min(row0 + 16 * NQ - 1, a.rows - 1) / a.group, tq - 1) + 1));
+    if (row0 / a.group >= tq) last_key = 0;
     const int chunks = (last_key + 31) / 32, share = (chunks + a.nsplit - 1) / a.nsplit;
     const int chunk0 = split * share, chunk1 = min(chunks, chunk0 + share);
 
@@ -272,7 +276,7 @@ void attention_few_kernel(AttnArgs a)
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
         const int r = row0 + 16 * t + x16, rc = min(r, a.rows - 1);
-        lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
+        lim[t] = a.causal ? len - tq + min(rc / a.group, tq - 1) + 1 : len;
         const char* qp = a.q + (int64_t)b * a.q_stride[0] + (int64_t)(rc / a.group) * a.q_stride[1] + (int64_t)(h * a.group + rc % a.group) * a.q_stride[2];
 #pragma unroll
         for (int u = 0; u < DP / 32; ++u) {
@@ -290,7 +294,7 @@ void attention_few_kernel(AttnArgs a)
         }
     }
 
-    const int first_lim = a.causal ? len - a.tq + row0 / a.group + 1 : 0x7fffffff;       // every row of this tile sees the keys below it
+    const int first_lim = a.causal ? len - tq + row0 / a.group + 1 : 0x7fffffff;         // every row of this tile sees the keys below it
 
     f32x4 o[NQ][F::NO];
     float m[NQ], l[NQ];
@@ -555,6 +559,10 @@ void attention_few_kernel(AttnArgs a)
                 for (int i = 0; i < 4; ++i) acc[i] = seen.instead_of(acc[i], i);
             }
         }
+        if (r / a.group >= tq) {
+            sum = 0.0f;
+            acc = f32x4{};
+        }
         if (a.nsplit > 1) {
             float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
             if (at == 0) { ws[0] = top; ws[1] = sum; }
@@ -645,10 +653,11 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
     const int place = place_of(a.n * a.kv_heads, a.tiles * a.nsplit, id);
     const int split = (int)(id % a.nsplit), tile = a.tiles - 1 - (int)(id / a.nsplit);   // (causal: the longest rows first)
     const int b = longest_first(a, place / a.kv_heads), h = place % a.kv_heads, bh = b * a.kv_heads + h;
-    const int len = keys_of(a, b), row0 = tile * MANY_ROWS * NR, wave_row0 = row0 + 32 * NR * wave;
+    const int len = keys_of(a, b), row0 = tile * MANY_ROWS * NR, wave_row0 = row0 + 32 * NR * wave, tq = queries_of<CODES>(a, b);
     int last_key = len;
-    if (a.causal) last_key = min(len, max(0, len - a.tq + min(row0 + MANY_ROWS * NR - 1, a.rows - 1) / a.group + 1));
-    const int first_lim = a.causal ? len - a.tq + row0 / a.group + 1 : 0x7fffffff;       // every row of this workgroup sees the keys below it
+    if (a.causal) last_key = min(len, max(0, len - tq + min(min(row0 + MANY_ROWS * NR - 1, a.rows - 1) / a.group, tq - 1) + 1));
+    if (row0 / a.group >= tq) last_key = 0;
+    const int first_lim = a.causal ? len - tq + row0 / a.group + 1 : 0x7fffffff;         // every row of this workgroup sees the keys below it
     const int all_tiles = (last_key + MANY_KEYS - 1) / MANY_KEYS, share = (all_tiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * share, t1 = min(all_tiles, t0 + share);
 
@@ -668,9 +677,9 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
             if constexpr (QTERMS == 2) cut_f16(w, qf[t][u]);
             else qf[t][u][0] = w;
         }
-        lim[t] = a.causal ? len - a.tq + rc / a.group + 1 : len;
+        lim[t] = a.causal ? len - tq + min(rc / a.group, tq - 1) + 1 : len;
     }
-    const int wave_first = a.causal ? len - a.tq + min(wave_row0, a.rows - 1) / a.group + 1 : 0x7fffffff;      // every row of this wave sees keys below it
+    const int wave_first = a.causal ? len - tq + min(min(wave_row0, a.rows - 1) / a.group, tq - 1) + 1 : 0x7fffffff;      // every row of this wave sees keys below it
 
     const char* kb = a.k + (int64_t)b * a.k_stride[0] + (int64_t)h * a.k_stride[2];
     const char* vb = a.v + (int64_t)b * a.v_stride[0] + (int64_t)h * a.v_stride[2];
@@ -1082,8 +1091,13 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
         const int r = wave_row0 + 32 * t + x32;
-        const float sum = halves_sum(l[t]);
+        float sum = halves_sum(l[t]);
         if (r >= a.rows) continue;
+        if (CODES && r / a.group >= tq) {
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) o[t][i] = f32x16{};
+        }
         if (a.nsplit > 1) {
             float* ws = a.ws + (((int64_t)split * a.n * a.kv_heads + bh) * a.rows + r) * (a.d + 4);
             if (half == 0) { ws[0] = m[t]; ws[1] = sum; }
@@ -1315,7 +1329,7 @@ int64_t asr_kv8_attention_workspace(int32_t n, int32_t tq, int32_t capacity, int
     return plan_of(n, tq, capacity, heads, kv_heads, d, dtype == ASR_F32 ? 3 : dtype == ASR_F16 ? 2 : 1).ws_bytes;
 }
 
-int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
+int asr_kv8_attention_counts(const asr_kv8_attention_args* a, const int32_t* counts, void* stream)
 {
     if (!a) return ops_fail(ASR_ERR_ARG, "null argument");
     if (const char* why = bad_sizes(a->n, a->tq, a->capacity, a->heads, a->kv_heads, a->d, 16)) return ops_fail(ASR_ERR_ARG, "kv8_attention: %s", why);
@@ -1336,7 +1350,7 @@ int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
     x.q = static_cast<const char*>(a->q); x.out = static_cast<char*>(a->out);
     x.k = reinterpret_cast<const char*>(a->k_cache); x.v = reinterpret_cast<const char*>(a->v_cache);
     x.k_scale = a->k_scale; x.v_scale = a->v_scale; x.scale_stride = a->capacity / ASR_KV8_BLOCK;
-    x.lens = a->lens;
+    x.lens = a->lens; x.counts = counts;
     for (int i = 0; i < 3; ++i) { x.q_stride[i] = a->q_stride[i] * size; x.out_stride[i] = a->out_stride[i] * size; }
     x.k_stride[0] = x.v_stride[0] = a->cache_stride[0];
     x.k_stride[1] = x.v_stride[1] = a->d;
@@ -1350,5 +1364,7 @@ int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream)
     if (a->dtype == ASR_BF16) return attend<ASR_BF16, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
     return attend<ASR_F16, KV_E4M3>("kv8_attention", x, p, a->workspace, a->workspace_bytes, s);
 }
+
+int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream) { return asr_kv8_attention_counts(a, nullptr, stream); }
 
 }  // extern "C"

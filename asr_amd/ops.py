@@ -35,13 +35,13 @@ _ATTEND = struct.Struct('@8P9q8if4x')
 _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle without the Stream object around it (1 us a call)
 
 
-def _call(fn, packed, device):
-    """fn(packed arguments) on the current stream of the device with this number."""
+def _call(fn, packed, device, *more):
+    """fn(packed arguments, more) on the current stream of the device with this number."""
     if device == torch.cuda.current_device():
-        rc = fn(packed, _raw_stream(device))
+        rc = fn(packed, *more, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(packed, _raw_stream(device))
+            rc = fn(packed, *more, _raw_stream(device))
     if rc:
         raise AsrError(rc, lib.asr_ops_last_error().decode('utf-8', 'replace'))
 
@@ -246,13 +246,16 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, lens, counts=None):
                        capacity, dtype), device)
 
 
-def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, scale=None, out=None):
+def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, scale=None, out=None, counts=None):
     """q [n, tq, heads, d] (float32, bfloat16 or float16) over the first lens[b] (int32 [n]) tokens of each sequence's cache ->
     [n, tq, heads, d] of q's type.  causal: query i is the sequence's token lens[b] - tq + i, which the cache already holds, and sees nothing behind
     itself.  A query with nothing to see gives zeros; what it does not see does not matter, NaN included.  Query head h reads key head
-    h // (heads // kv_heads); scale defaults to 1 / sqrt(d); d is a multiple of 16 up to 128."""
+    h // (heads // kv_heads); scale defaults to 1 / sqrt(d); d is a multiple of 16 up to 128.
+
+    counts (int32 [n]; None: tq for all): sequence b's queries are its first counts[b], like the new tokens of kv8_append with the same counts, and query
+    i of a causal call is its token lens[b] - counts[b] + i; the rows behind them give zeros.  Without it the queries of every sequence end with its newest token."""
     name = 'kv8_attention'
-    device = _device(name, q, k_cache, v_cache, k_scale, v_scale, lens, out)
+    device = _device(name, q, k_cache, v_cache, k_scale, v_scale, lens, out, counts)
     n, kv_heads, capacity, d, cs = _cache(name, k_cache, v_cache, k_scale, v_scale)
     dtype = _DTYPES.get(q.dtype)
     if dtype is None:
@@ -262,11 +265,13 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, sca
     _, tq, heads, _ = q.shape
     qs = _rows(name, 'q', q, (n, tq, heads, d))
     _counts(name, 'lens', lens, n)
+    if counts is not None:
+        _counts(name, 'counts', counts, n)
     out = _output(name, q, out)
     size = _kv8_workspace(n, tq, capacity, heads, kv_heads, d, dtype)
     ws = q.new_empty((size,), dtype=torch.uint8) if size else None
-    _call(lib.asr_kv8_attention,
+    _call(lib.asr_kv8_attention_counts,
           _ATTEND.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                        lens.data_ptr(), 0 if ws is None else ws.data_ptr(), *qs, *out.stride()[:3], cs[0], cs[1], size, n, tq, heads, kv_heads,
-                       d, capacity, dtype, 1 if causal else 0, (d or 1) ** -0.5 if scale is None else scale), device)
+                       d, capacity, dtype, 1 if causal else 0, (d or 1) ** -0.5 if scale is None else scale), device, 0 if counts is None else counts.data_ptr())
     return out

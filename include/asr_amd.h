@@ -365,7 +365,7 @@ typedef struct asr_kv8_append_args {
 int asr_kv8_append(const asr_kv8_append_args* a, void* stream);
 
 /* asr_cross_attention with the cache above for keys and values; lens[b] tokens are valid (taken as 0 below 0, as the capacity above it).
- * causal: query i of sequence b is its token lens[b] - tq + i and sees nothing behind itself (the cache already holds the tq newest tokens; a
+ * causal: query i of sequence b is its token lens[b] - tq + i, its LAST row the newest token, and sees nothing behind itself (the cache already holds the tq newest tokens; a
  * query with nothing to see gives 0; NaN in later tokens does not reach it).  Codes are multiplied exactly on the 16-bit matrix instruction; a q of f16 or f32 enters as
  * two or three bf16 terms, so nothing of it is lost; probabilities as two, or three with f32. */
 typedef struct asr_kv8_attention_args {
@@ -385,6 +385,10 @@ typedef struct asr_kv8_attention_args {
 } asr_kv8_attention_args;
 int64_t asr_kv8_attention_workspace(int32_t n, int32_t tq, int32_t capacity, int32_t heads, int32_t kv_heads, int32_t d, int32_t dtype);
 int asr_kv8_attention(const asr_kv8_attention_args* a, void* stream);
+
+/* The same where sequences have different numbers of queries, as after asr_kv8_append with counts: sequence b's are its first counts[b] (int32 [n] on the device; taken as 0
+ * below 0 and as tq above it; null: all tq), the rest of its rows give 0 whatever their q.  causal: query i is the sequence's token lens[b] - counts[b] + i. */
+int asr_kv8_attention_counts(const asr_kv8_attention_args* a, const int32_t* counts, void* stream);
 
 /* ---- instrumentation ---------------------------------------------------------------------- */
 
