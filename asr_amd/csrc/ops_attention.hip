@@ -609,11 +609,12 @@ __device__ inline u32x2 lds_read_transposed(const __attribute__((address_space(3
     return __builtin_bit_cast(u32x2, x);
 }
 // 16 bytes a lane from memory to LDS, the wave's 1024 in lane order from `lds` on; done when the wave has waited for its memory operations.  (The
-// builtin would have every later LDS read wait for it, as the compiler cannot tell the buffers apart.)
+// builtin would have every later LDS read wait for it, as the compiler cannot tell the buffers apart.  The place in LDS is an operand in m0, so the compiler sets that
+// register and knows what is in it; its read needs a wait state.)
 __device__ inline uint32_t lds_at(char* p) { return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p); }
 __device__ inline void load_to_lds(mem p, uint32_t at)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(at) : "memory");
 }
 __device__ inline void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ inline float halves_max(float x)
