@@ -8,8 +8,9 @@
 
 The work is queued on the current stream of the tensors' device, like torch's own operators: nothing here waits for the GPU, results are
 torch tensors of the caller's allocator, and a call can be captured into a graph.  Tensors that were made on another stream
-need that stream waited for first (and `record_stream`), as with every torch operator.  There is no backward pass: tensors that
-require gradients are refused while gradients are recorded.
+need that stream waited for first (and `record_stream`), as with every torch operator.  There is no backward pass and no
+forward-mode derivative: tensors that require gradients while these are recorded, and tensors with a tangent, are refused.  So are
+tensors without memory of their own (fake ones, wrappers).
 
 Wrong types, shapes or devices raise ValueError; what the library itself refuses raises `AsrError`.
 """
@@ -19,6 +20,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import AsrError, lib
 
@@ -32,6 +34,8 @@ _APPEND = struct.Struct('@8P8q6i')
 _ATTEND = struct.Struct('@8P9q8if4x')
 
 
+_Tensor = torch.Tensor
+_plain = torch._C._disabled_torch_dispatch_impl       # what tensors have for __torch_dispatch__ that are no wrappers
 _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle without the Stream object around it (1 us a call)
 
 
@@ -48,24 +52,33 @@ def _call(fn, packed, device, *more):
 
 # The checks below run before every call: a message is only put together when it is needed.
 def _refused(name, *tensors):
-    """Why these tensors (None entries are skipped) cannot be used together: they are not all on one GPU, or want gradients."""
+    """Why these tensors cannot be used together - they have no memory, are not all on one GPU, want derivatives - or None."""
     device = tensors[0].get_device()
+    if any(type(t).__torch_dispatch__ is not _plain for t in tensors):
+        return ValueError('%s: tensors must have memory of their own (no fake tensors, no wrappers)' % name)
     if device < 0:
         return ValueError('%s: tensors must be in GPU memory' % name)
-    if any(t is not None and t.get_device() != device for t in tensors):
+    if any(t.get_device() != device for t in tensors):
         return ValueError('%s: all tensors must be on one device' % name)
-    return ValueError('%s has no backward pass: detach its inputs or call it under torch.no_grad()' % name)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return ValueError('%s has no backward pass: detach its inputs or call it under torch.no_grad()' % name)
+    if torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return ValueError('%s has no forward-mode derivative: call it on the primals (torch.autograd.forward_ad.unpack_dual)' % name)
+    return None
 
 
 def _device(name, *tensors):
     """The number of the one device that holds all tensors (None entries are skipped)."""
     device = tensors[0].get_device()
     grads = torch.is_grad_enabled()
+    odd = device < 0 or forward_ad._current_level >= 0                  # (tensors have tangents inside a dual level alone)
     for t in tensors:
-        if t is not None and (t.get_device() != device or (grads and t.requires_grad)):
-            raise _refused(name, *tensors)
-    if device < 0:
-        raise _refused(name, *tensors)
+        if t is not None and (t.get_device() != device or (grads and t.requires_grad) or type(t) is not _Tensor):
+            odd = True
+    if odd:
+        error = _refused(name, *[t for t in tensors if t is not None])
+        if error is not None:
+            raise error
     return device
 
 
