@@ -36,6 +36,7 @@ _ATTEND = struct.Struct('@8P9q8if4x')
 
 _Tensor = torch.Tensor
 _plain = torch._C._disabled_torch_dispatch_impl       # what tensors have for __torch_dispatch__ that are no wrappers
+_changed = torch._C._increment_version                 # tensors that were written in place: autograd is told, as torch's own operators do
 _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle without the Stream object around it (1 us a call)
 
 
@@ -192,6 +193,7 @@ def cross_attention(q, k, v, lens=None, pad=None, scale=None, out=None):
         if (pad.dtype is not torch.bool and pad.dtype is not torch.uint8) or pad.shape != (n, tk) or (tk > 1 and pad.stride(1) != 1):
             raise ValueError('%s: pad must be bool or uint8 [n, tk], contiguous in tk' % name)
         pad_stride = pad.stride(0)
+    given = out is not None
     out = _output(name, q, out)
     size = _cross_workspace(n, tq, tk, heads, kv_heads, d, dtype)
     ws = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -199,6 +201,8 @@ def cross_attention(q, k, v, lens=None, pad=None, scale=None, out=None):
           _CROSS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lens is None else lens.data_ptr(),
                       0 if pad is None else pad.data_ptr(), 0 if ws is None else ws.data_ptr(), *qs, *ks, *vs, *out.stride()[:3],
                       pad_stride, size, n, tq, tk, heads, kv_heads, d, dtype, (d or 1) ** -0.5 if scale is None else scale), device)
+    if given:
+        _changed((out,))
     return out
 
 
@@ -257,6 +261,7 @@ def kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, lens, counts=None):
           _APPEND.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                        lens.data_ptr(), 0 if counts is None else counts.data_ptr(), *ks, *vs, cs[0], cs[1], n, new, kv_heads, d,
                        capacity, dtype), device)
+    _changed((k_cache, v_cache, k_scale, v_scale))
 
 
 def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, scale=None, out=None, counts=None):
@@ -280,6 +285,7 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, sca
     _counts(name, 'lens', lens, n)
     if counts is not None:
         _counts(name, 'counts', counts, n)
+    given = out is not None
     out = _output(name, q, out)
     size = _kv8_workspace(n, tq, capacity, heads, kv_heads, d, dtype)
     ws = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -287,4 +293,6 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, sca
           _ATTEND.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                        lens.data_ptr(), 0 if ws is None else ws.data_ptr(), *qs, *out.stride()[:3], cs[0], cs[1], size, n, tq, heads, kv_heads,
                        d, capacity, dtype, 1 if causal else 0, (d or 1) ** -0.5 if scale is None else scale), device, 0 if counts is None else counts.data_ptr())
+    if given:
+        _changed((out,))
     return out
