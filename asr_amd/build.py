@@ -12,6 +12,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')
 LIB = os.path.join(CSRC, 'libasr_amd.so')
+RECIPE = os.path.abspath(__file__)                    # the flags are in it: objects older than this file are compiled again
 SOURCES = ['gemm_f32.hip', 'gemm_split.hip', 'rowops.hip', 'frontend.hip', 'attention.hip', 'ops_rows.hip', 'ops_attention.hip', 'engine.hip']
 HEADERS = ['asr_common.h', 'gemm_epilogue.h', 'ops_common.h', os.path.join('..', '..', 'include', 'asr_amd.h')]
 # Packed float32 instructions are off: the compiler makes them from ordinary float code, and some of their forms have given wrong
@@ -42,7 +43,7 @@ def build_library(force=False, verbose=True):
         s = os.path.join(CSRC, src)
         o = os.path.join(CSRC, src.replace('.hip', '.o'))
         objs.append(o)
-        if force or _stale(o, [s] + hdrs):
+        if force or _stale(o, [s, RECIPE] + hdrs):
             jobs.append([hipcc] + FLAGS + ['-c', s, '-o', o])
 
     def run(cmd):
