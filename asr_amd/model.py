@@ -172,8 +172,8 @@ class Engine(object):
 
     def score(self, X, Y, top=0):
         """Token by token what `loss` adds up: X float32 [n, t, d], Y int32 [n, ty] (0 = padding) -> (logprob [n, ty], entropy [n, ty],
-        top_logprobs [n, ty, top], top_tokens [n, ty, top]): log p of every target given the ones before it (0 for padding), the
-        entropy of its distribution and the `top` (at most 32) most likely tokens there (`asr_score`)."""
+        top_logprobs [n, ty, top], top_tokens [n, ty, top]): log p of every target given the ones before it (0 for padding and negative targets, NaN for
+        one beyond the vocabulary; `loss` counts these as 0), the entropy of its distribution and the `top` (at most 32) most likely tokens there (`asr_score`)."""
         X = _lib.f32(X)
         Y = _lib.i32(Y)
         if X.ndim != 3 or Y.ndim != 2 or Y.shape[0] != X.shape[0]:

@@ -154,8 +154,9 @@ int asr_loss(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d,
 /* What asr_loss adds up, token by token, and how sure the model was: the same teacher-forced pass over Y int32 [n, ty] (0 = padding), then for
  * every position logprob [n, ty] = log p(Y | the targets before it, X), entropy [n, ty] of that distribution, and top_tokens / top_logprobs [n, ty, top] =
  * its `top` (0 .. 32) most likely tokens, ties to the lower one (asr_token_logprobs below).  Padding has log probability 0, and the distribution's
- * entropy and alternatives like every position.  Confidence of hypotheses and rescoring of n-best lists need these; the reference only
- * has the sum (model.py:350-360: loss_sum = minus the sum of logprob over Y != 0). */
+ * entropy and alternatives like every position.  A target outside the vocabulary is not a token of the model: a negative one has log probability 0 like
+ * padding, one >= dst_vocab_size gives NaN, where asr_loss counts both as 0 (the one-hot row of such a label is all zeros).  Confidence of hypotheses and rescoring of n-best lists need these; the reference only
+ * has the sum (model.py:350-360: loss_sum = minus the sum of logprob over the targets 0 < Y < dst_vocab_size). */
 int asr_score(asr_handle* h, const float* X, int32_t n, int32_t t, int32_t d, const int32_t* Y, int32_t ty, int32_t top, float* logprob,
               float* entropy, float* top_logprobs, int32_t* top_tokens);
 
