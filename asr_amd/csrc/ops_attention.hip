@@ -115,6 +115,12 @@ __device__ inline float groups_sum(float x)
 // nearly all tiles skip the scaling of the sums.  It starts finite, so that no difference with it is NaN.  A float16 P is relative down to 2^-14 and 0 below 2^-25: there m stays
 // LIFT below the maximum that it follows, so that the largest P of a row is 2^7 to 2^15 and keys 22 nats below it still count (a largest one of 1 lost those 17 nats below).
 constexpr float SLACK = 8.0f, LIFT16 = 7.0f, NO_MAX = -3.0e38f;
+// a b rounded, never one operation with what is added to it
+__device__ inline float product(float a, float b)
+{
+#pragma clang fp contract(off)
+    return a * b;
+}
 __device__ inline float rescale(float m_old, float m_new) { return __builtin_amdgcn_exp2f(m_old - m_new); }
 
 // An infinity in an admitted V: a term of P that is 0, or of the other sign than the first, makes NaN of it, as does scaling what was summed by 0, and the cut of a float32 one.
@@ -408,7 +414,7 @@ void attention_few_kernel(AttnArgs a)
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[t][j] = s[t][j >> 2][j & 3] * a.c;
+            for (int j = 0; j < 8; ++j) p[t][j] = product(s[t][j >> 2][j & 3], a.c);
             if (mask != 0xffffffffu) {
                 asm volatile("");                                              // (a branch, not selects in every chunk)
 #pragma unroll
@@ -827,13 +833,15 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         for (int i = 1; i < 16; ++i) x = fmaxf(x, s[i]);
         return halves_max(x);
     };
-    uint64_t grow = 0;                                                               // the lanes whose rows' maximum has grown
-    constexpr float LIFT = F16 ? LIFT16 : 0.0f;
-    const auto grown_by = [&](int r) __attribute__((always_inline)) { return fmaf(top[r], c, -m[r]); };         // (what the exponentials take: none is above it)
+    // The exponentials take fma(s, c, -m) with m a rounded product: none is above that of the maximum but by half a step of m.  Where that step is more than a few hundredths (FAR) scores
+    // are multiplied, rounded like m, and m subtracted: their steps would otherwise pass the range of P.
+    constexpr float LIFT = F16 ? LIFT16 : 0.0f, FAR = 0x1p20f;
+    uint64_t far = 0, grow = 0;                                                      // the lanes whose rows' m is that far; ... or whose maximum has grown
+    const auto grown_by = [&](int r) __attribute__((always_inline)) { return fmaf(top[r], c, -m[r]); };
     const auto grows = [&]() __attribute__((always_inline)) {
         bool x = grown_by(0) > SLACK + LIFT;
         if (NR > 1) x |= grown_by(NR - 1) > SLACK + LIFT;
-        return __ballot(x);
+        return __ballot(x) | far;
     };
     // soft-max and output of half `sub` of tile t from its scores s with their maxima `top`, and the scores of the half behind it.  The products are laid out
     // as slots, one for each, and between them, in the order in which it is to be issued (the compiler left to itself puts all products on one
@@ -859,16 +867,27 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
             }
             grow = grows();
         }
+        float factor = c;
         if (grow) {
+            bool is_far = false;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                const float grown = grown_by(r) > SLACK + LIFT ? top[r] * c - LIFT : m[r], f = rescale(m[r], grown);
+                const float t = product(top[r], c), grown = fmaxf(grown_by(r), t - m[r]) > SLACK + LIFT ? t - LIFT : m[r], f = rescale(m[r], grown);
                 m[r] = grown;
+                is_far |= fabsf(grown) > FAR && grown != NO_MAX;
                 l[r] *= f;
 #pragma unroll
                 for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) o[r][i][j] *= f;
+            }
+            far = __ballot(is_far);
+            if (far) {
+                factor = 1.0f;
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[r][i] = product(s[r][i], c);
             }
         }
         const auto v_frag = [&](int q) __attribute__((always_inline)) {
@@ -890,7 +909,7 @@ template <int QT, int KVT, int DP, int NR, bool FULL> __global__ __launch_bounds
         const auto key_of = [](int e) { return 8 * (e / (8 * NR)) + e % 8; };
         // values whose exponential is taken by the end of slot w: all before the output's second half
         const auto taken = [](int w) { return w < 0 ? 0 : VALUES * (w + 1) >= VALUES * (SLOTS * 3 / 2 - 1) ? VALUES : (VALUES * (w + 1) + SLOTS * 3 / 2 - 2) / (SLOTS * 3 / 2 - 1); };
-        const auto begin = [&](int e) __attribute__((always_inline)) { x[row_of(e)][key_of(e)] = fmaf(s[row_of(e)][key_of(e)], c, -m[row_of(e)]); };
+        const auto begin = [&](int e) __attribute__((always_inline)) { x[row_of(e)][key_of(e)] = fmaf(s[row_of(e)][key_of(e)], factor, -m[row_of(e)]); };
         const auto between = [&](int w) __attribute__((always_inline)) {
             if (w >= SLOTS * 3 / 2) return;
 #pragma unroll
