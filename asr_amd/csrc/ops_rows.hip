@@ -388,12 +388,14 @@ __device__ inline int kv8_exponent(uint32_t magnitude)          // of a finite f
 }
 __device__ inline float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
 
+// the largest code under a scale of 2^e: 448, but under 2^120, which only magnitudes from 1.75 * 2^127 need, 256 would already stand for 2^128
+__device__ inline float kv8_most(int e) { return e < 120 ? 448.0f : 240.0f; }
 // four e4m3 codes of x * inv: infinities saturate (a code conversion of anything beyond 464 would give NaN), NaN passes
-__device__ inline float kv8_clamp(float x) { return x != x ? x : __builtin_amdgcn_fmed3f(x, -448.0f, 448.0f); }
-__device__ inline uint32_t kv8_codes(float x0, float x1, float x2, float x3)
+__device__ inline float kv8_clamp(float x, float most) { return x != x ? x : __builtin_amdgcn_fmed3f(x, -most, most); }
+__device__ inline uint32_t kv8_codes(float x0, float x1, float x2, float x3, float most)
 {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(kv8_clamp(x0), kv8_clamp(x1), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(kv8_clamp(x2), kv8_clamp(x3), r, true);
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(kv8_clamp(x0, most), kv8_clamp(x1, most), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(kv8_clamp(x2, most), kv8_clamp(x3, most), r, true);
 }
 
 struct Kv8AppendArgs {
@@ -464,12 +466,12 @@ template <int DT, int NT, int ITEMS> __global__ __launch_bounds__(NT) void kv8_a
                 const uint32_t c = old[i];
                 typedef float f32x2 __attribute__((ext_vector_type(2)));
                 const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-                old[i] = kv8_codes(p[0] * f, p[1] * f, q[0] * f, q[1] * f);
+                old[i] = kv8_codes(p[0] * f, p[1] * f, q[0] * f, q[1] * f, kv8_most(e));
             }
         }
         e = max(e, e_was);
     }
-    const float inv = pow2f(-e);
+    const float inv = pow2f(-e), largest = kv8_most(e);
     uint8_t* to = codes + (lo - first) * a.d;
 #pragma unroll
     for (int u = 0; u < ITEMS; ++u) {
@@ -479,7 +481,7 @@ template <int DT, int NT, int ITEMS> __global__ __launch_bounds__(NT) void kv8_a
         Elem<DT>::unpack(raw[u], y);
         uint32_t w[PER / 4];
 #pragma unroll
-        for (int j = 0; j < PER / 4; ++j) w[j] = kv8_codes(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
+        for (int j = 0; j < PER / 4; ++j) w[j] = kv8_codes(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv, largest);
         uint32_t* out = reinterpret_cast<uint32_t*>(to + i * PER);
 #pragma unroll
         for (int j = 0; j < PER / 4; ++j) out[j] = w[j];

@@ -321,9 +321,10 @@ int asr_token_logprobs(const asr_token_logprobs_args* a, void* stream);
  * of one utterance are query rows (tq = beams): nothing orders the queries.
  * q, out: [n, tq, heads, d], k, v: [n, tk, kv_heads, d] of one type, d contiguous, every other stride free but such that each row starts on
  * 16 bytes; out may not overlap the inputs.  bf16 and f16 are multiplied as they are; f32 is cut into three bf16 terms (exact) of whose nine products the six
- * above 2^-24 are taken, so an infinity in an f32 query or admitted key gives NaN.  Infinities in admitted values are the result of their column, whatever their weight (both
- * signs: NaN).  Scores, soft-max statistics and sums are float32.  With bf16 and f16
- * the probabilities enter as two terms of that type (2^-17 of each is lost, or 2^-22 and at most 2^-32 of the row's largest), whatever the number of rows.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
+ * above 2^-24 are taken, so an infinity in an f32 query or admitted key gives NaN.  Infinities in admitted values are the result of their column, whatever
+ * their weight (both signs: NaN).  Scores, soft-max statistics and sums are float32; sums are divided at the end, so values beyond 2^119 / tk may pass
+ * float32 on the way.  With bf16 and f16 the probabilities enter as two terms of that type (2^-17 of each is lost, or 2^-22 and at most 2^-32 of the
+ * row's largest), whatever the number of rows.  heads % kv_heads == 0, d % 8 == 0, 8 <= d <= 128. */
 typedef struct asr_cross_attention_args {
     const void *q, *k, *v;
     void* out;
@@ -349,7 +350,8 @@ int asr_cross_attention(const asr_cross_attention_args* a, void* stream);
  * sequence with lens[b] < 0 or counts[b] <= 0 is left alone).  The scale of a block is the smallest power of two, 2^-100 at the least, with which
  * every finite magnitude it was made for stays within 448, the largest e4m3 value; a value is rounded once, to the nearest code, halves to
  * even.  A block that held tokens before (lens[b] inside it) keeps its scale or takes the larger one its new tokens need; its older tokens are then
- * coded again under it.  Infinities are held as +-448, NaN stays NaN; neither counts for a scale.  Nothing else is written: blocks
+ * coded again under it.  Infinities are held as +-448, NaN stays NaN; neither counts for a scale.  Under a scale of 2^120, which magnitudes
+ * from 1.75 * 2^127 (2.98e38) need, the largest code is 240: 256 would stand for 2^128.  Nothing else is written: blocks
  * without new tokens, and positions behind the last one, stay as they are.  No two sequences may share cache memory, nor may K and V.
  * k, v: [n, new_tokens, kv_heads, d], any asr_dtype, rows on 16 bytes.  d % 16 == 0, 16 <= d <= 128; capacity % ASR_KV8_BLOCK == 0. */
 typedef struct asr_kv8_append_args {
