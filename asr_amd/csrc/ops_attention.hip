@@ -154,7 +154,7 @@ __device__ inline int keys_of(const AttnArgs& a, int b) { return a.lens ? min(ma
 // Workgroup `id` -> (sequence, K/V head), and what is left of id for its row tile and share, `per` of them for each.  Consecutive workgroups go round the
 // eight XCDs, each with an L2 of its own: all workgroups of one (sequence, head) go to one XCD, next to each other, so that its keys are read into one
 // L2 once; an XCD gets another head of each sequence (the same head's rows, a power of two apart where the heads of a token lie side by side, share a few of
-// the L2's channels).  Eight sequences, eight heads of 128, 24 row tiles: 328 us with the tiles next to each other, 368 with the heads.
+// the L2's channels).  Eight sequences, eight heads of 128, 24 row tiles, probabilities of one term: 328 us with the tiles next to each other, 368 with the heads.
 __device__ inline int place_of(int nbh, int per, int64_t& id)
 {
     int bh;
@@ -173,7 +173,8 @@ __device__ inline int place_of(int nbh, int per, int64_t& id)
 template <bool CODES> __device__ inline int queries_of(const AttnArgs& a, int b) { return CODES && a.counts ? min(max(a.counts[b], 0), a.tq) : a.tq; }
 
 // The sequence that is number `at` when the longest come first (at itself where that would not matter or take too long): the last workgroups of a launch
-// are then short ones (16 x 200 queries over 1500 states of half to full length: 41.5 -> 38 us; one token over 64 caches of up to 2048: 45.7 -> 42.9).  Finding it
+// are then short ones (16 x 200 queries over 1500 states of half to full length: 45.2 -> 43.1 us; 64 x 80 over caches of up to 2048 of 8 heads: 61.5 -> 57; one token over 64
+// such caches of 16 heads: 45.7 -> 42.9).  Finding it
 // costs up to half a microsecond a workgroup, too much for few rows over short keys (64 x 10 queries over 334 states: 15.5 -> 16.4 us).
 __device__ inline int longest_first(const AttnArgs& a, int at)
 {
@@ -591,13 +592,13 @@ void attention_few_kernel(AttnArgs a)
 // ---- many rows: the waves of a workgroup share tiles of keys in LDS ------------------------------------------------------
 // 16-bit products only, the probabilities as two terms like those of few rows (codes with a float16 q: q as two bf16 terms too, which keep its bits).  One term would
 // save a third of the products and round every probability to 8 bits: as much error as the result's own rounding adds (8 x 768 queries of 32 heads over 4001 states of 8
-// heads of 128: 440 us and 0.0017 of the result with two, 322 us and 0.0023 with one).  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
+// heads of 128: 450 us and 0.0017 of the result with two, 328 us and 0.0023 with one).  A workgroup has 128 rows (NR = 1) or 256, 32 NR for each of its four waves, and walks over tiles of 64 keys that it stages into LDS
 // (K three buffers, V two: the next tiles' loads are in flight while this one is used, one barrier a tile; codes become bf16 on the way, times their block's
 // scale).  32 x 32 x 16 products: S^T = K q^T has a row in each lane of 32 and lane half; O^T = V^T P^T takes V^T from LDS with the transposing read
 // (four keys of one column a lane) and P^T straight from the accumulators: what a term lacks is exact in float32 and becomes the next one.
 // The 16-byte chunks of a row are permuted by its number (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4), by pairs of rows where rows are half
 // as long): both kinds of read then meet every bank evenly.  Rows of 16-bit values as long as the tile go from memory to LDS directly.
-// What bounds it: instructions.  A tile is 48 products (1536 cycles of the matrix pipe) and some 290 vector instructions a wave and row tile; products of one
+// What bounds it: instructions.  A tile is 48 products (1536 cycles of the matrix pipe) and some 300 vector instructions a wave and row tile; products of one
 // wave run beside the vector instructions of both waves of a SIMD, but a wave alone issues only every 7 cycles.
 constexpr int MANY_WAVES = 4, MANY_ROWS = 32 * MANY_WAVES, MANY_KEYS = 64;               // (MANY_ROWS: for each row tile of a wave)
 
@@ -1214,13 +1215,14 @@ Plan plan_of(int64_t n, int64_t tq, int64_t tk, int64_t heads, int64_t kv_heads,
     p.many = terms < 3 && p.rows > 64;
     if (p.many) {
         // two row tiles a wave where its registers hold them and workgroups of twice the rows still give every compute unit two, without many idle rows (8 x 512
-        // queries of 32 heads over 4096 states of 8 heads of 64: 230 us with one, 220 with two, though those spill some twenty registers; heads of 128 would leave one
+        // queries of 32 heads over 4096 states of 8 heads of 64: 230 us with one, 220 with two, though those spill eleven registers, over codes 22; heads of 128 would leave one
         // wave a SIMD)
         const int64_t tiles = (p.rows + MANY_ROWS - 1) / MANY_ROWS;
         p.nq = terms == 1 && d == 64 && (tiles % 2 == 0 || tiles >= 8) && n * kv_heads * ((tiles + 1) / 2) >= 512 ? 2 : 1;
         p.tiles = (int)((tiles + p.nq - 1) / p.nq);
-        // shares of at least eight tiles, with few workgroups of four where there are twelve (joining them is a launch: 4 x 61 queries of 16 heads over 1000 states,
-        // 64 workgroups, 24.7 us in one share and 18.4 in three; 8 x 61 over 800, 128 workgroups, 16.8 and 19.9; 2 x 100 over 1500, 32 workgroups, 19.5 and 15.5)
+        // shares of at least eight tiles, with few workgroups of four where there are twelve (joining them is a launch: 4 x 100 queries of 16 heads over 1000 states,
+        // 64 workgroups, 22.8 us with eight and 18.8 with four; 2 x 100 over 1500, 32 workgroups, 22.8 and 16.3; 4 x 80 of 8 heads of 128 over 1000, 29 and 19.6; 8 x 100 over
+        // 800, 128 workgroups, 19.7 and 23.8)
         const int64_t wgs = n * kv_heads * p.tiles, most = wgs <= 64 && tk >= 12 * MANY_KEYS ? tk / (MANY_KEYS * 4) : tk / (MANY_KEYS * 8);
         int64_t split = wgs > 0 ? 512 / wgs : 1;
         if (split > most) split = most;
