@@ -98,9 +98,11 @@ def _rows(name, what, t, dims):
     return a, b, c
 
 
-def _output(name, q, out):
+def _output(name, q, out, k=None, v=None):
     if out is None:
         return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is not None and out.numel() and out.data_ptr() in (k.data_ptr(), v.data_ptr()):
+        raise ValueError('%s: out must not overlap k or v' % name)
     if out.dtype != q.dtype or out.shape != q.shape:
         raise ValueError('%s: out must have the shape and type of q' % name)
     if not all(s > 0 or n <= 1 for s, n in zip(out.stride(), out.shape)):
@@ -172,7 +174,8 @@ def cross_attention(q, k, v, lens=None, pad=None, scale=None, out=None):
     softmax(scale q k^T) v per sequence and head, query head h reading key head h // (heads // kv_heads); scale defaults to
     1 / sqrt(d).  Admitted are the first lens[b] (int32 [n]; None: all) states of which pad[b] (bool or uint8 [n, tk]; None: none) is zero; whatever
     stands in the others does not matter, and a sequence without any gives zeros.  Beams of an utterance are its query rows.
-    d is a multiple of 8 up to 128; rows start on 16 bytes; other strides are free (k and v may be the halves of one projection)."""
+    d is a multiple of 8 up to 128; rows start on 16 bytes; other strides are free (k and v may be the halves of one projection).  out must not overlap the
+    inputs (the same memory as k or v is refused)."""
     name = 'cross_attention'
     device = _device(name, q, k, v, lens, pad, out)
     dtype = _DTYPES.get(q.dtype)
@@ -194,7 +197,7 @@ def cross_attention(q, k, v, lens=None, pad=None, scale=None, out=None):
             raise ValueError('%s: pad must be bool or uint8 [n, tk], contiguous in tk' % name)
         pad_stride = pad.stride(0)
     given = out is not None
-    out = _output(name, q, out)
+    out = _output(name, q, out, k, v)
     size = _cross_workspace(n, tq, tk, heads, kv_heads, d, dtype)
     ws = q.new_empty((size,), dtype=torch.uint8) if size else None
     _call(lib.asr_cross_attention,
@@ -271,7 +274,7 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, lens, causal=False, sca
     h // (heads // kv_heads); scale defaults to 1 / sqrt(d); d is a multiple of 16 up to 128.
 
     counts (int32 [n]; None: tq for all): sequence b's queries are its first counts[b], like the new tokens of kv8_append with the same counts, and query
-    i of a causal call is its token lens[b] - counts[b] + i; the rows behind them give zeros.  Without it the queries of every sequence end with its newest token."""
+    i of a causal call is its token lens[b] - counts[b] + i; the rows behind them give zeros.  Without it the queries of every sequence end with its newest token.  out must not overlap the inputs."""
     name = 'kv8_attention'
     device = _device(name, q, k_cache, v_cache, k_scale, v_scale, lens, out, counts)
     n, kv_heads, capacity, d, cs = _cache(name, k_cache, v_cache, k_scale, v_scale)
